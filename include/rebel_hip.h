@@ -277,6 +277,53 @@ typedef struct {
 int rbl_engine_timing(rbl_engine* e, int stride);
 int rbl_engine_stats(rbl_engine* e, rbl_kernel_stats* out, int reset);
 
+/* ---- training operators: what lies between the matrix products of Net2 (cfvpy/models.py:41-53) and between the backward pass
+ * and the optimizer (cfvpy/selfplay.py:418-439).  All pointers named _dev are device memory of `device`; the work is enqueued on
+ * `stream` (a hipStream_t of that device; NULL: its default stream) and nothing waits for it.  No state is kept from call to
+ * call: what a call needs beside its operands is the workspace that the caller gives it, which no two calls in flight may
+ * share.  Everything here may be captured into a HIP graph.  Results do not depend on timing: there are no atomics. ---- */
+enum { RBL_F32 = 0, RBL_F16 = 1, RBL_BF16 = 2 };
+enum { RBL_ACT_NONE = 0, RBL_ACT_GELU = 1 /* x/2 (1 + erf(x / sqrt 2)) */ };
+
+/* Layer normalisation over the last dimension: x is [rows][cols], z = (x - mean) / sqrt(variance + eps) * weight + bias per
+ * row, y = z or GELU(z).  Statistics, sums and the activation are computed in f32; the result is rounded once to `dtype`. */
+typedef struct {
+  int64_t rows, cols;          /* rows >= 0; 1 <= cols <= 2^30 */
+  int64_t x_stride, dy_stride; /* elements from one row to the next (0: every row is the same memory); y and dx are dense */
+  int32_t dtype;               /* of x, y, dy, dx: RBL_F32, RBL_F16, RBL_BF16 */
+  int32_t param_dtype;         /* of weight, bias and their gradients: RBL_F32 or `dtype` */
+  int32_t activation;          /* RBL_ACT_* */
+  float eps;
+} rbl_layer_norm_shape;
+int64_t rbl_layer_norm_workspace(const rbl_layer_norm_shape* s, int backward); /* bytes; -1: error */
+/* weight_dev / bias_dev may be NULL (1 / 0).  stats_dev: NULL, or [rows][2] f32 that receives mean and 1 / sqrt(variance + eps)
+ * for the backward pass. */
+int rbl_layer_norm_forward(int device, const rbl_layer_norm_shape* s, const void* x_dev, const void* weight_dev,
+                           const void* bias_dev, void* y_dev, float* stats_dev, void* workspace_dev, int64_t workspace_bytes,
+                           void* stream);
+/* dx_dev, dweight_dev, dbias_dev: the gradients of x, weight and bias; each may be NULL (not wanted).  The parameters' gradients
+ * are sums over the rows in f32, in an order that depends on the shape alone.  rows = 0 gives zeros. */
+int rbl_layer_norm_backward(int device, const rbl_layer_norm_shape* s, const void* dy_dev, const void* x_dev,
+                            const void* weight_dev, const void* bias_dev, const float* stats_dev, void* dx_dev,
+                            void* dweight_dev, void* dbias_dev, void* workspace_dev, int64_t workspace_bytes, void* stream);
+
+/* The norm of many gradients taken as one vector, and their clipping to a bound: factor = min(1, max_norm / (norm + 1e-6)).
+ * Sums are held in f64 and the norm is rounded to f32 once.  A NaN anywhere makes the norm NaN. */
+typedef struct {
+  void* data_dev; /* numel consecutive elements; the tensors must not overlap when they are scaled */
+  int64_t numel;
+  int32_t dtype; /* RBL_F32, RBL_F16, RBL_BF16, each tensor its own */
+} rbl_grad;
+enum { RBL_NORM_1 = 1, RBL_NORM_2 = 2, RBL_NORM_INF = 3 };
+int64_t rbl_grad_workspace(const rbl_grad* grads, int n); /* bytes; -1: error */
+int rbl_grad_norm(int device, const rbl_grad* grads, int n, int norm, float* norm_dev, void* workspace_dev,
+                  int64_t workspace_bytes, void* stream);
+/* the norm, then every gradient times the factor, in place; norm_dev receives the norm before clipping */
+int rbl_grad_clip(int device, const rbl_grad* grads, int n, int norm, double max_norm, float* norm_dev, void* workspace_dev,
+                  int64_t workspace_bytes, void* stream);
+/* every gradient times the factor of a norm that is there already */
+int rbl_grad_scale(int device, const rbl_grad* grads, int n, double max_norm, const float* norm_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

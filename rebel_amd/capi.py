@@ -32,6 +32,8 @@ SYMBOLS = [
     "rbl_selfplay_root_dedup_served",
     "rbl_selfplay_state", "rbl_selfplay_on_device", "rbl_selfplay_device_examples", "rbl_selftest_device_rng",
     "rbl_engine_timing", "rbl_engine_stats",
+    "rbl_layer_norm_workspace", "rbl_layer_norm_forward", "rbl_layer_norm_backward",
+    "rbl_grad_workspace", "rbl_grad_norm", "rbl_grad_clip", "rbl_grad_scale",
 ]
 
 
@@ -48,6 +50,20 @@ class MlpWeights(C.Structure):
                 ("b", C.POINTER(C.POINTER(C.c_float))), ("ln_w", C.POINTER(C.POINTER(C.c_float))),
                 ("ln_b", C.POINTER(C.POINTER(C.c_float))), ("w_out", C.POINTER(C.c_float)),
                 ("b_out", C.POINTER(C.c_float)), ("ln_eps", C.c_float)]
+
+
+class LayerNormShape(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("cols", C.c_int64), ("x_stride", C.c_int64), ("dy_stride", C.c_int64),
+                ("dtype", C.c_int32), ("param_dtype", C.c_int32), ("activation", C.c_int32), ("eps", C.c_float)]
+
+
+class Grad(C.Structure):
+    _fields_ = [("data_dev", C.c_void_p), ("numel", C.c_int64), ("dtype", C.c_int32)]
+
+
+F32, F16, BF16 = 0, 1, 2  # element types of the training operators
+ACT_NONE, ACT_GELU = 0, 1
+NORM_1, NORM_2, NORM_INF = 1, 2, 3
 
 
 class KernelStats(C.Structure):
@@ -161,6 +177,14 @@ def lib():
         "rbl_selftest_device_rng": (C.c_int, [C.c_int, C.c_int32, C.c_int, C.c_int, dp, C.c_int, dp]),
         "rbl_engine_timing": (C.c_int, [vp, C.c_int]),
         "rbl_engine_stats": (C.c_int, [vp, C.POINTER(KernelStats), C.c_int]),
+        "rbl_layer_norm_workspace": (C.c_int64, [C.POINTER(LayerNormShape), C.c_int]),
+        "rbl_layer_norm_forward": (C.c_int, [C.c_int, C.POINTER(LayerNormShape), vp, vp, vp, vp, vp, vp, C.c_int64, vp]),
+        "rbl_layer_norm_backward": (C.c_int, [C.c_int, C.POINTER(LayerNormShape), vp, vp, vp, vp, vp, vp, vp, vp, vp, C.c_int64,
+                                              vp]),
+        "rbl_grad_workspace": (C.c_int64, [C.POINTER(Grad), C.c_int]),
+        "rbl_grad_norm": (C.c_int, [C.c_int, C.POINTER(Grad), C.c_int, C.c_int, vp, vp, C.c_int64, vp]),
+        "rbl_grad_clip": (C.c_int, [C.c_int, C.POINTER(Grad), C.c_int, C.c_int, C.c_double, vp, vp, C.c_int64, vp]),
+        "rbl_grad_scale": (C.c_int, [C.c_int, C.POINTER(Grad), C.c_int, C.c_double, vp, vp]),
     }
     assert sorted(sig) == sorted(SYMBOLS)
     for name, (res, args) in sig.items():

@@ -1912,6 +1912,10 @@ int guard(F&& f) {
 }
 }  // namespace
 
+namespace rbl {
+void set_last_error(const char* what) { g_err = what; }  // train_kernels.h
+}  // namespace rbl
+
 extern "C" {
 
 const char* rbl_last_error(void) { return g_err.c_str(); }

@@ -1,0 +1,287 @@
+// rebel_amd/csrc/train_module.cc -- the training operators of the C ABI (include/rebel_hip.h) on torch tensors, with their
+// gradients.  rebel_amd/training.py is the public face.
+//
+// Work is enqueued on torch's current stream of the tensors' device; outputs, statistics and workspaces come from torch's
+// allocator on that stream, so a captured graph keeps its own and nothing is shared between two calls.
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <cmath>
+#include <optional>
+#include <stdexcept>
+#include <vector>
+
+#include "../../include/rebel_hip.h"
+
+namespace {
+
+using torch::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+void check(int status) {
+  if (status != 0) throw std::runtime_error(rbl_last_error());
+}
+// A refused argument is a ValueError
+template <class... Words>
+void require(bool ok, const Words&... words) {
+  if (!ok) throw std::invalid_argument(c10::str(words...));
+}
+
+// -1: not one of the operators' types
+int element_type(at::ScalarType t) {
+  return t == at::kFloat ? RBL_F32 : t == at::kHalf ? RBL_F16 : t == at::kBFloat16 ? RBL_BF16 : -1;
+}
+
+void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+
+// The elements from one row of the last dimension to the next, where all rows lie at one distance; -1 where they do not, or
+// where a row's elements do not lie side by side.
+int64_t row_stride(const Tensor& t) {
+  const auto sizes = t.sizes();
+  const auto strides = t.strides();
+  const int d = (int)sizes.size() - 1;
+  if (t.numel() == 0) return sizes[d];
+  if (sizes[d] > 1 && strides[d] != 1) return -1;
+  int64_t step = -1, rows = 1;  // of the dimensions behind i that have more than one entry
+  for (int i = d - 1; i >= 0; --i) {
+    if (sizes[i] == 1) continue;
+    if (step >= 0 && strides[i] != step * rows) return -1;
+    if (step < 0) step = strides[i];
+    rows *= sizes[i];
+  }
+  return step < 0 ? sizes[d] : step;
+}
+
+Tensor with_rows(const Tensor& t) { return row_stride(t) < 0 ? t.contiguous() : t; }
+
+Tensor workspace(const Tensor& like, int64_t bytes) {
+  check(bytes < 0);
+  return bytes == 0 ? Tensor() : at::empty({bytes}, like.options().dtype(at::kByte));
+}
+void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+rbl_layer_norm_shape shape_of(const Tensor& x, const Tensor& w, const Tensor& b, double eps, int64_t activation) {
+  rbl_layer_norm_shape s{};
+  s.cols = x.size(-1);
+  s.rows = s.cols ? x.numel() / s.cols : 0;
+  s.x_stride = s.dy_stride = s.cols;
+  s.dtype = element_type(x.scalar_type());
+  s.param_dtype = w.defined() ? element_type(w.scalar_type()) : b.defined() ? element_type(b.scalar_type()) : RBL_F32;
+  s.activation = (int32_t)activation;
+  s.eps = (float)eps;
+  return s;
+}
+
+void check_arguments(const Tensor& x, const Tensor& w, const Tensor& b) {
+  require(x.defined() && x.dim() >= 1, "layer_norm: x needs at least one dimension");
+  require(element_type(x.scalar_type()) >= 0, "layer_norm: x must be float32, float16 or bfloat16, not ", x.scalar_type());
+  require(x.size(-1) >= 1, "layer_norm: the last dimension of x is empty");
+  for (const Tensor* p : {&w, &b}) {
+    if (!p->defined()) continue;
+    require(p->dim() == 1 && p->size(0) == x.size(-1), "layer_norm: weight and bias must have shape [", x.size(-1),
+                "], the last dimension of x, not ", p->sizes());
+    require(p->scalar_type() == at::kFloat || p->scalar_type() == x.scalar_type(),
+                "layer_norm: weight and bias must be float32 or of x's type, not ", p->scalar_type());
+    require(p->device() == x.device(), "layer_norm: weight and bias must be on x's device ", x.device(), ", not ",
+                p->device());
+  }
+  require(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(),
+              "layer_norm: weight and bias must have one type");
+  require(x.layout() == at::kStrided, "layer_norm: x must be a dense tensor");
+  require(x.is_cuda(), "layer_norm: x must be on the GPU: there is no CPU path");
+}
+
+// y, and the rows' statistics if `stats` is not null
+Tensor forward(const Tensor& x, const Tensor& w, const Tensor& b, double eps, int64_t activation, Tensor* stats) {
+  c10::DeviceGuard guard(x.device());
+  rbl_layer_norm_shape s = shape_of(x, w, b, eps, activation);
+  s.x_stride = row_stride(x);
+  Tensor y = at::empty(x.sizes(), x.options());
+  if (stats) *stats = at::empty({s.rows, 2}, x.options().dtype(at::kFloat));
+  Tensor space = workspace(x, rbl_layer_norm_workspace(&s, 0));
+  check(rbl_layer_norm_forward(x.get_device(), &s, data(x), data(w), data(b), data(y), stats ? stats->data_ptr<float>() : nullptr,
+                               data(space), space.defined() ? space.numel() : 0, stream_of(x)));
+  return y;
+}
+
+// A leaf's gradient is added up on the stream on which its accumulator was made.  If an earlier, eager graph of the same leaf
+// is still alive, a backward pass that is being captured would run into that other stream, and the process would end.
+void refuse_foreign_accumulator(const Tensor& t) {
+  if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!node) return;
+  const auto s = node->stream();
+  require(s && *s == c10::hip::getCurrentHIPStream(t.get_device()).unwrap(),
+              "layer_norm: a graph that was made outside this capture still holds a leaf of this call; delete its outputs before "
+              "capturing (or make it on the capturing stream)");
+}
+
+class LayerNormFn : public torch::autograd::Function<LayerNormFn> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x_in, const OptTensor& w_in, const OptTensor& b_in,
+                        double eps, int64_t activation) {
+    const Tensor x = with_rows(x_in), w = w_in ? w_in->contiguous() : Tensor(), b = b_in ? b_in->contiguous() : Tensor();
+    Tensor stats;
+    Tensor y = ::forward(x, w, b, eps, activation, &stats);
+    // the bias comes back only where the activation's slope depends on it
+    ctx->save_for_backward({x, w, activation == RBL_ACT_NONE ? Tensor() : b, stats});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["activation"] = activation;
+    ctx->saved_data["given"] = (int64_t)(w.defined() + 2 * b.defined());
+    ctx->saved_data["param_type"] =
+        (int64_t)(w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : at::kFloat);
+    return y;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    if (at::GradMode::is_enabled())
+      throw std::runtime_error("layer_norm: its gradient has no gradient of its own (create_graph)");
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &stats = saved[3];
+    c10::DeviceGuard guard(x.device());
+    const Tensor dy = with_rows(grads[0]);
+    rbl_layer_norm_shape s = shape_of(x, w, b, ctx->saved_data["eps"].toDouble(), ctx->saved_data["activation"].toInt());
+    const auto param_type = (at::ScalarType)ctx->saved_data["param_type"].toInt();
+    s.param_dtype = element_type(param_type);
+    s.x_stride = row_stride(x);
+    s.dy_stride = row_stride(dy);
+    Tensor dx, dw, db;
+    if (ctx->needs_input_grad(0)) dx = at::empty(x.sizes(), x.options());
+    // the edges count only the parameters that were given
+    const int64_t given = ctx->saved_data["given"].toInt();
+    const bool has_w = given & 1, has_b = given & 2;
+    if (has_w && ctx->needs_input_grad(1)) dw = at::empty({s.cols}, x.options().dtype(param_type));
+    if (has_b && ctx->needs_input_grad(1 + has_w)) db = at::empty({s.cols}, x.options().dtype(param_type));
+    Tensor space = workspace(x, rbl_layer_norm_workspace(&s, 1));
+    check(rbl_layer_norm_backward(x.get_device(), &s, data(dy), data(x), data(w), data(b), stats.data_ptr<float>(), data(dx),
+                                  data(dw), data(db), data(space), space.defined() ? space.numel() : 0, stream_of(x)));
+    return {dx, dw, db, Tensor(), Tensor()};
+  }
+};
+
+Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int64_t activation) {
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  check_arguments(x, w, b);
+  const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) ||
+                                                   (b.defined() && b.requires_grad()));
+  if (!grad)
+    return forward(with_rows(x), w.defined() ? w.contiguous() : w, b.defined() ? b.contiguous() : b, eps, activation, nullptr);
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+    for (const Tensor* t : {&x, &w, &b}) refuse_foreign_accumulator(*t);
+  return LayerNormFn::apply(x, w.defined() ? OptTensor(w) : OptTensor(), b.defined() ? OptTensor(b) : OptTensor(), eps, activation);
+}
+
+// ------------------------------------------------------------------------------------------------ gradient norm
+struct Gradients {
+  std::vector<rbl_grad> list;
+  std::vector<std::pair<Tensor, Tensor>> copies;  // tensors with gaps: (the tensor, its values side by side)
+  Tensor any;
+};
+
+Gradients gather(const std::vector<Tensor>& tensors, bool scaled) {
+  Gradients g;
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+  for (const Tensor& t : tensors) {
+    require(t.defined(), "gradients: a tensor is undefined");
+    require(t.layout() == at::kStrided, "gradients: sparse gradients are not supported");
+    const int type = element_type(t.scalar_type());
+    require(type >= 0, "gradients: must be float32, float16 or bfloat16, not ", t.scalar_type());
+    if (!g.any.defined()) g.any = t;
+    require(t.device() == g.any.device(), "gradients: all must be on one device, not on ", g.any.device(), " and ", t.device());
+    if (t.numel() == 0) continue;
+    Tensor dense = t;
+    if (!t.is_non_overlapping_and_dense()) {
+      dense = t.contiguous();
+      if (scaled) {
+        // the furthest element; no two may share their memory
+        int64_t reach = 1;
+        for (int64_t i = 0; i < t.dim(); ++i) {
+          require(t.size(i) == 1 || t.stride(i) != 0, "gradients: a tensor that repeats its memory cannot be scaled in place");
+          reach += (t.size(i) - 1) * t.stride(i);
+        }
+        g.copies.emplace_back(t, dense);
+        const auto at = (uintptr_t)t.data_ptr();
+        spans.emplace_back(at, at + reach * t.element_size());
+      }
+    } else if (scaled) {
+      const auto at = (uintptr_t)t.data_ptr();
+      spans.emplace_back(at, at + t.numel() * t.element_size());
+    }
+    g.list.push_back({dense.data_ptr(), dense.numel(), type});
+    if (!scaled && dense.data_ptr() != t.data_ptr()) g.copies.emplace_back(t, dense);  // alive until the launch
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    require(spans[i].first >= spans[i - 1].second, "gradients: two of them share memory (the same tensor twice?)");
+  if (g.any.defined()) require(g.any.is_cuda(), "gradients: must be on the GPU: there is no CPU path");
+  return g;
+}
+
+int norm_kind(double p) {
+  const int kind = p == 1.0 ? RBL_NORM_1 : p == 2.0 ? RBL_NORM_2 : p == INFINITY ? RBL_NORM_INF : 0;
+  require(kind, "gradients: norm_type must be 1, 2 or inf, not ", p);
+  return kind;
+}
+
+Tensor norm_of(const Gradients& g, int kind) {
+  c10::DeviceGuard guard(g.any.device());
+  Tensor norm = at::empty({}, g.any.options().dtype(at::kFloat).layout(at::kStrided));
+  const int n = (int)g.list.size();
+  Tensor space = workspace(g.any, rbl_grad_workspace(g.list.data(), n));
+  check(rbl_grad_norm(g.any.get_device(), g.list.data(), n, kind, norm.data_ptr<float>(), data(space),
+                      space.defined() ? space.numel() : 0, stream_of(g.any)));
+  return norm;
+}
+
+Tensor grad_norm(const std::vector<Tensor>& tensors, double norm_type) {
+  at::NoGradGuard no_grad;
+  const int kind = norm_kind(norm_type);
+  const Gradients g = gather(tensors, false);
+  return g.any.defined() ? norm_of(g, kind) : at::zeros({});
+}
+
+Tensor clip_grad_norm(const std::vector<Tensor>& parameters, double max_norm, double norm_type, bool error_if_nonfinite) {
+  at::NoGradGuard no_grad;
+  const int kind = norm_kind(norm_type);
+  require(max_norm >= 0, "gradients: max_norm must be a number >= 0, not ", max_norm);
+  std::vector<Tensor> grads;
+  grads.reserve(parameters.size());
+  for (const Tensor& p : parameters)
+    if (p.grad().defined()) grads.push_back(p.grad());
+  const Gradients g = gather(grads, true);
+  if (!g.any.defined()) return at::zeros({});
+  c10::DeviceGuard guard(g.any.device());
+  const int n = (int)g.list.size();
+  Tensor norm;
+  if (error_if_nonfinite) {
+    require(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
+                "gradients: error_if_nonfinite looks at the norm on the host, which a capture cannot do");
+    norm = norm_of(g, kind);
+    const float value = norm.item<float>();
+    if (!std::isfinite(value))
+      throw std::runtime_error(c10::str("gradients: the total norm of order ", norm_type, " is ", value,
+                                        ", so they were not clipped (error_if_nonfinite)"));
+    check(rbl_grad_scale(g.any.get_device(), g.list.data(), n, max_norm, norm.data_ptr<float>(), stream_of(g.any)));
+  } else {
+    norm = at::empty({}, g.any.options().dtype(at::kFloat));
+    Tensor space = workspace(g.any, rbl_grad_workspace(g.list.data(), n));
+    check(rbl_grad_clip(g.any.get_device(), g.list.data(), n, kind, max_norm, norm.data_ptr<float>(), data(space),
+                        space.defined() ? space.numel() : 0, stream_of(g.any)));
+  }
+  for (const auto& c : g.copies) c.first.copy_(c.second);
+  return norm;
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("layer_norm", &layer_norm, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("eps"), py::arg("activation"),
+        py::call_guard<py::gil_scoped_release>());
+  m.def("grad_norm", &grad_norm, py::arg("tensors"), py::arg("norm_type"), py::call_guard<py::gil_scoped_release>());
+  m.def("clip_grad_norm", &clip_grad_norm, py::arg("parameters"), py::arg("max_norm"), py::arg("norm_type"),
+        py::arg("error_if_nonfinite"), py::call_guard<py::gil_scoped_release>());
+}

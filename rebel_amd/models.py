@@ -26,13 +26,21 @@ class GELU(nn.Module):
 
 
 class Net2(nn.Module):
-    def __init__(self, *, num_faces, num_dice, n_hidden=256, use_layer_norm=False, dropout=0, n_layers=3):
+    """native=True: LayerNorm and the GELU behind it run as one HIP kernel, forward and backward (training.LayerNorm); needs
+    use_layer_norm.  Same parameters, state_dict and scripted form; a net that is not scripted then runs on the GPU only."""
+
+    def __init__(self, *, num_faces, num_dice, n_hidden=256, use_layer_norm=False, dropout=0, n_layers=3, native=False):
         super().__init__()
+        if native and not use_layer_norm:
+            raise ValueError("Net2: native=True replaces the LayerNorm and its GELU, so it needs use_layer_norm=True")
         n_in = input_size(num_faces, num_dice)
         slots, width = [], n_in
-        act = GELU()
+        act = GELU() if not native else nn.Sequential()
+        if native:
+            from rebel_amd import training  # needs the built libraries; the plain net does not
         for _ in range(n_layers):
             slots += [nn.Linear(width, n_hidden),
+                      training.LayerNorm(n_hidden, activation="gelu") if native else
                       nn.LayerNorm(n_hidden) if use_layer_norm else nn.Sequential(),
                       act,
                       nn.Dropout(dropout) if dropout > 0 else nn.Sequential()]
