@@ -6,8 +6,8 @@
 // and, with g = dy (GELU: g = dy (Phi(z) + z phi(z)), phi the density):
 //     db = sum_rows g     dw = sum_rows g h     dx = r (g w - sum(g w) / n - h sum(g w h) / n)
 //
-// Simple form: a workgroup to a row, which it walks three times (the row stays in the caches); the parameters' gradients by a
-// second kernel that walks columns.  h is computed again from x and the two statistics of the row, so nothing else is kept
+// Backward, simple form: a workgroup to a row, which it walks twice (the row stays in the caches); the parameters' gradients by
+// a second kernel that walks columns.  h is computed again from x and the two statistics of the row, so nothing else is kept
 // between the passes.
 #include "train_kernels.h"
 
@@ -60,7 +60,9 @@ struct NormArgs {
   void *y, *dx, *dw, *db;
   float* stats;    // [rows][2]: mean, 1 / sqrt(variance + eps)
   int64_t rows, x_stride, dy_stride;
+  float* partial;  // workspace
   int cols;
+  int chunks;     // of a row that is longer than a workgroup's registers
   int param_f32;  // the parameters' type: f32, or the rows' type
   float eps;
 };
@@ -93,36 +95,244 @@ __device__ __forceinline__ void sum_block(float& p, float& q, float (*slots)[2])
   q = (slots[0][1] + slots[1][1]) + (slots[2][1] + slots[3][1]);
 }
 
-template <class T, int ACT>
-__global__ __launch_bounds__(kThreads) void layer_norm_forward_kernel(NormArgs a) {
-  __shared__ float slots[kThreads / 64][2];
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const T* x = (const T*)a.x + row * a.x_stride;
+// V consecutive elements in one access: 16 bytes, at the alignment of an element (the memory pipe takes any).
+template <class T, int V>
+struct Pack {
+  typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+};
+
+// Which columns a thread of a row's group owns.  Vector v covers [v V, v V + V); the one that would reach past the row is moved
+// back to end with it and leaves out (`skip`) what the vector before it owns already, so every load is a whole one and none needs
+// a branch.  A vector that lies wholly past the row skips everything.
+template <int V, int TPR, bool EVEN>
+struct Place {
+  int col, skip;
+  Place() = default;
+  __device__ __forceinline__ Place(int t, int k, int cols) {
+    const int at = (t + k * TPR) * V;
+    col = EVEN || at + V <= cols ? at : cols - V;
+    skip = EVEN ? 0 : at - col;
+  }
+  __device__ __forceinline__ bool owns(int i) const { return EVEN || i >= skip; }
+  __device__ __forceinline__ bool any() const { return EVEN || skip < V; }
+};
+
+template <class T, int V>
+__device__ __forceinline__ void load_params(const NormArgs& a, const void* p, int col, float missing, float (&out)[V]) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = missing;
+  } else if (a.param_f32) {
+    const auto v = *(const typename Pack<float, V>::type*)((const float*)p + col);
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = v[i];
+  } else {
+    const auto v = *(const typename Pack<T, V>::type*)((const T*)p + col);
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = (float)v[i];
+  }
+}
+
+// Sums of N numbers over the TPR threads that share a row, the same bits in each of them.  Groups of 16 and 64 stay in their
+// wavefront; larger ones (whole workgroups) exchange one number per wavefront through LDS.  Two buffers in turn make one barrier
+// per call enough: a wavefront can be at most one call ahead of another.
+template <int TPR, int N>
+__device__ __forceinline__ void sum_group(float (&v)[N], float* slots, int& turn) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = TPR == 16 ? sum16(v[i]) : sum64(v[i]);
+  if constexpr (TPR > 64) {
+    constexpr int W = TPR / 64;
+    float* s = slots + turn * 2 * W;
+    turn ^= 1;
+    if (threadIdx.x % 64 == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[i * W + threadIdx.x / 64] = v[i];
+    }
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float t = s[i * W];
+#pragma unroll
+      for (int w = 1; w < W; ++w) t += s[i * W + w];
+      v[i] = t;
+    }
+  }
+}
+
+// Mean and 1 / sqrt(variance + eps) of the row whose elements the group's threads hold.  The variance is the mean square of
+// the deviations from the rounded mean; their sum, which would be zero but for that rounding, corrects both.
+template <int V, int TPR, int K, bool EVEN>
+__device__ __forceinline__ void statistics(const float (&x)[K][V], const Place<V, TPR, EVEN> (&at)[K], int cols, float eps,
+                                           float* slots, int& turn, float& mean, float& r) {
+  float s[1] = {0};
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[0] += at[k].owns(i) ? x[k][i] : 0.0f;
+  sum_group<TPR>(s, slots, turn);
+  const float n = (float)cols, first = s[0] / n;
+  float d[2] = {0, 0};
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float e = at[k].owns(i) ? x[k][i] - first : 0.0f;
+      d[0] += e;
+      d[1] = __builtin_fmaf(e, e, d[1]);
+    }
+  sum_group<TPR>(d, slots, turn);
+  mean = first + d[0] / n;
+  float variance = (d[1] - d[0] * d[0] / n) / n;
+  variance = variance < 0 ? 0 : variance;  // NaN stays
+  r = 1.0f / __builtin_sqrtf(variance + eps);
+}
+
+// Forward, a row in the registers of TPR threads (K vectors of V elements each): read once, written once.
+template <class T, int V, int TPR, int K, bool EVEN, int ACT>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_forward_kernel(NormArgs a) {
+  constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
+  typedef typename Pack<T, V>::type vec;
+  __shared__ float slots[TPR > 64 ? 4 * TPR / 64 : 1];
+  int turn = 0;
+  const int t = threadIdx.x % TPR;
+  Place<V, TPR, EVEN> at[K];
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  if (row >= a.rows) return;  // whole groups; of a group of more than a wavefront there is one to a workgroup
+  constexpr bool KEEP = K * V <= 16;  // the parameters stay in registers
+  float w[K][V], b[K][V];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    at[k] = Place<V, TPR, EVEN>(t, k, a.cols);
+    if (KEEP) {
+      load_params<T, V>(a, a.w, at[k].col, 1.0f, w[k]);
+      load_params<T, V>(a, a.b, at[k].col, 0.0f, b[k]);
+    }
+  }
+  vec next[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) next[k] = *(const vec*)((const T*)a.x + row * a.x_stride + at[k].col);
+  for (; row < a.rows; row += step) {
+    float x[K][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[k][i] = (float)next[k][i];
+    const int64_t ahead = row + step < a.rows ? row + step : row;  // the next row is on its way while this one is computed
+#pragma unroll
+    for (int k = 0; k < K; ++k) next[k] = *(const vec*)((const T*)a.x + ahead * a.x_stride + at[k].col);
+    float mean, r;
+    statistics<V, TPR, K, EVEN>(x, at, a.cols, a.eps, slots, turn, mean, r);
     T* y = (T*)a.y + row * a.cols;
-    float s = 0, zero = 0;
-    for (int c = threadIdx.x; c < a.cols; c += kThreads) s += (float)x[c];
-    sum_block(s, zero, slots);
-    // the deviations from the rounded mean: their sum corrects it
-    const float first = s / a.cols;
-    float off = 0, square = 0;
-    for (int c = threadIdx.x; c < a.cols; c += kThreads) {
-      const float d = (float)x[c] - first;
-      off += d;
-      square = __builtin_fmaf(d, d, square);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (!KEEP) {
+        load_params<T, V>(a, a.w, at[k].col, 1.0f, w[k]);
+        load_params<T, V>(a, a.b, at[k].col, 0.0f, b[k]);
+      }
+      vec out;
+#pragma unroll
+      for (int i = 0; i < V; ++i) out[i] = (T)activate<ACT>(__builtin_fmaf((x[k][i] - mean) * r, w[k][i], b[k][i]));
+      // a moved-back vector writes again what its neighbour writes, the same values
+      if (at[k].any()) *(vec*)(y + at[k].col) = out;
     }
-    sum_block(off, square, slots);
-    const float mean = first + off / a.cols;
-    float variance = (square - off * off / a.cols) / a.cols;
-    variance = variance < 0 ? 0 : variance;  // NaN stays
-    const float r = 1.0f / __builtin_sqrtf(variance + a.eps);
-    for (int c = threadIdx.x; c < a.cols; c += kThreads) {
-      const float h = ((float)x[c] - mean) * r;
-      y[c] = (T)activate<ACT>(__builtin_fmaf(h, param<T>(a, a.w, c, 1.0f), param<T>(a, a.b, c, 0.0f)));
+    if (a.stats && t == 0) *(float2*)(a.stats + 2 * row) = make_float2(mean, r);
+  }
+}
+
+// Rows that are longer than a workgroup's registers: chunks of kChunk vectors, each with its own mean and sum of squared
+// deviations, which the second kernel joins (Chan's formula) before it normalises its chunk.
+constexpr int kChunkK = 4;
+template <int V>
+constexpr int chunk_cols() { return kThreads * kChunkK * V; }
+
+template <class T, int V>
+__global__ __launch_bounds__(kThreads) void layer_norm_chunk_statistics_kernel(NormArgs a) {
+  typedef typename Pack<T, V>::type vec;
+  __shared__ float slots[4 * kThreads / 64];
+  int turn = 0;
+  for (int64_t item = blockIdx.x; item < a.rows * a.chunks; item += gridDim.x) {
+    const int64_t row = item / a.chunks;
+    const int chunk = (int)(item - row * a.chunks), begin = chunk * chunk_cols<V>();
+    const int cols = min(a.cols - begin, chunk_cols<V>());
+    const T* x = (const T*)a.x + row * a.x_stride + begin;
+    float s[1] = {0}, e[2] = {0, 0};
+    float v[kChunkK][V];
+    bool own[kChunkK][V];
+#pragma unroll
+    for (int k = 0; k < kChunkK; ++k) {
+      // the last chunk may be shorter than a vector: it reads back into the one before
+      const int at = (threadIdx.x + k * kThreads) * V, col = at + V <= cols ? at : cols - V;
+      const vec p = *(const vec*)(x + col);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        own[k][i] = i >= at - col;
+        v[k][i] = own[k][i] ? (float)p[i] : 0.0f;
+        s[0] += v[k][i];
+      }
     }
-    if (a.stats && threadIdx.x == 0) {
-      a.stats[2 * row] = mean;
-      a.stats[2 * row + 1] = r;
+    sum_group<kThreads>(s, slots, turn);
+    const float n = (float)cols, first = s[0] / n;
+#pragma unroll
+    for (int k = 0; k < kChunkK; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float d = own[k][i] ? v[k][i] - first : 0.0f;
+        e[0] += d;
+        e[1] = __builtin_fmaf(d, d, e[1]);
+      }
+    sum_group<kThreads>(e, slots, turn);
+    if (threadIdx.x == 0) *(float2*)(a.partial + 2 * item) = make_float2(first + e[0] / n, e[1] - e[0] * e[0] / n);
+  }
+}
+
+// Every wavefront joins the chunks' statistics for itself.
+template <int V>
+__device__ __forceinline__ void join_chunks(const NormArgs& a, int64_t row, float& mean, float& r) {
+  const float2* p = (const float2*)a.partial + row * a.chunks;
+  const int lane = threadIdx.x % 64;
+  const float pivot = p[0].x, n = (float)a.cols;
+  float s = 0, q = 0;
+  for (int c = lane; c < a.chunks; c += 64) s += (p[c].x - pivot) * (float)min(a.cols - c * chunk_cols<V>(), chunk_cols<V>());
+  mean = pivot + sum64(s) / n;
+  for (int c = lane; c < a.chunks; c += 64) {
+    const float d = p[c].x - mean;
+    q += __builtin_fmaf(d * d, (float)min(a.cols - c * chunk_cols<V>(), chunk_cols<V>()), p[c].y);
+  }
+  const float variance = sum64(q) / n;
+  r = 1.0f / __builtin_sqrtf((variance < 0 ? 0 : variance) + a.eps);
+}
+
+template <class T, int V, int ACT>
+__global__ __launch_bounds__(kThreads) void layer_norm_chunk_forward_kernel(NormArgs a) {
+  typedef typename Pack<T, V>::type vec;
+  for (int64_t item = blockIdx.x; item < a.rows * a.chunks; item += gridDim.x) {
+    const int64_t row = item / a.chunks;
+    const int begin = (int)(item - row * a.chunks) * chunk_cols<V>();
+    const int cols = min(a.cols - begin, chunk_cols<V>());
+    const T* x = (const T*)a.x + row * a.x_stride + begin;
+    T* y = (T*)a.y + row * a.cols + begin;
+    vec p[kChunkK];
+    int col[kChunkK];
+#pragma unroll
+    for (int k = 0; k < kChunkK; ++k) {
+      const int at = (threadIdx.x + k * kThreads) * V;
+      col[k] = at + V <= cols ? at : cols - V;
+      p[k] = *(const vec*)(x + col[k]);
     }
+    float mean, r;
+    join_chunks<V>(a, row, mean, r);
+#pragma unroll
+    for (int k = 0; k < kChunkK; ++k) {
+      float w[V], b[V];
+      load_params<T, V>(a, a.w, begin + col[k], 1.0f, w);
+      load_params<T, V>(a, a.b, begin + col[k], 0.0f, b);
+      vec out;
+#pragma unroll
+      for (int i = 0; i < V; ++i) out[i] = (T)activate<ACT>(__builtin_fmaf(((float)p[k][i] - mean) * r, w[i], b[i]));
+      if ((threadIdx.x + k * kThreads) * V - col[k] < V) *(vec*)(y + col[k]) = out;
+    }
+    if (a.stats && begin == 0 && threadIdx.x == 0) *(float2*)(a.stats + 2 * row) = make_float2(mean, r);
   }
 }
 
@@ -179,11 +389,48 @@ __global__ __launch_bounds__(kThreads) void layer_norm_dparam_kernel(NormArgs a)
 
 unsigned row_grid(int64_t rows) { return (unsigned)(rows < 16384 ? rows : 16384); }
 
+constexpr int kCus = 256;
+
+template <class T, int V, int TPR, int K, int ACT>
+void forward_rows(NormArgs a, hipStream_t st) {
+  constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
+  // as many workgroups as the chip holds at once, each with its share of the rows
+  const int64_t need = (a.rows + RPB - 1) / RPB, most = (int64_t)kCus * (2048 / NT);
+  const void* kernel = a.cols == TPR * K * V ? (const void*)layer_norm_forward_kernel<T, V, TPR, K, true, ACT>
+                                             : (const void*)layer_norm_forward_kernel<T, V, TPR, K, false, ACT>;
+  void* args[] = {&a};
+  launch(kernel, (unsigned)(need < most ? need : most), NT, args, st);
+}
+
+// The widest row that a workgroup holds in its registers, in vectors
+constexpr int kMostVectors = 4096;
+
+template <class T>
+int chunk_count(int cols) {
+  constexpr int V = 16 / sizeof(T);
+  return (cols + chunk_cols<V>() - 1) / chunk_cols<V>();
+}
+
 template <class T, int ACT>
 void run_forward(NormArgs a, hipStream_t st) {
+  constexpr int V = 16 / sizeof(T);
   if (a.rows == 0) return;
+  const int vectors = (a.cols + V - 1) / V;
+  if (a.cols < V) return forward_rows<T, 1, 16, 1, ACT>(a, st);
+  if (vectors <= 16) return forward_rows<T, V, 16, 1, ACT>(a, st);
+  if (vectors <= 64) return forward_rows<T, V, 64, 1, ACT>(a, st);
+  if (vectors <= 128) return forward_rows<T, V, 64, 2, ACT>(a, st);
+  if (vectors <= 256) return forward_rows<T, V, 64, 4, ACT>(a, st);
+  if (vectors <= 512) return forward_rows<T, V, 256, 2, ACT>(a, st);
+  if (vectors <= 1024) return forward_rows<T, V, 256, 4, ACT>(a, st);
+  if (vectors <= 2048) return forward_rows<T, V, 1024, 2, ACT>(a, st);
+  if (vectors <= kMostVectors) return forward_rows<T, V, 1024, 4, ACT>(a, st);
+  a.chunks = chunk_count<T>(a.cols);
+  const int64_t items = a.rows * a.chunks;
+  const unsigned grid = (unsigned)(items < 1 << 20 ? items : 1 << 20);
   void* args[] = {&a};
-  launch((const void*)layer_norm_forward_kernel<T, ACT>, row_grid(a.rows), kThreads, args, st);
+  launch((const void*)layer_norm_chunk_statistics_kernel<T, V>, grid, kThreads, args, st);
+  launch((const void*)layer_norm_chunk_forward_kernel<T, V, ACT>, grid, kThreads, args, st);
 }
 template <class T, int ACT>
 void run_backward(NormArgs a, hipStream_t st) {
@@ -204,6 +451,18 @@ void check(const rbl_layer_norm_shape* s) {
     throw std::runtime_error("layer norm: unknown activation");
   if (s->x_stride < 0 || s->dy_stride < 0) throw std::runtime_error("layer norm: strides must not be negative");
   if (s->rows > 0 && s->rows > ((int64_t)1 << 60) / s->cols) throw std::runtime_error("layer norm: rows x cols is too large");
+}
+
+int64_t forward_workspace(const rbl_layer_norm_shape& s) {
+  const int size = s.dtype == RBL_F32 ? 4 : 2, v = 16 / size;
+  if (s.cols <= (int64_t)kMostVectors * v) return 0;
+  const int64_t chunk = kThreads * kChunkK * v;
+  return s.rows * ((s.cols + chunk - 1) / chunk) * 2 * (int64_t)sizeof(float);
+}
+
+void check_workspace(int64_t need, const void* workspace, int64_t bytes) {
+  if (bytes < need || (need > 0 && !workspace))
+    throw std::runtime_error("layer norm: the workspace must hold " + std::to_string(need) + " bytes");
 }
 
 NormArgs args_of(const rbl_layer_norm_shape& s) {
@@ -239,7 +498,7 @@ int64_t rbl_layer_norm_workspace(const rbl_layer_norm_shape* s, int backward) {
   int64_t bytes = -1;
   rbl::train_entry([&] {
     rbl::check(s);
-    bytes = 0;
+    bytes = backward ? 0 : rbl::forward_workspace(*s);
   });
   return bytes;
 }
@@ -256,6 +515,8 @@ int rbl_layer_norm_forward(int device, const rbl_layer_norm_shape* s, const void
     a.b = bias_dev;
     a.y = y_dev;
     a.stats = stats_dev;
+    a.partial = (float*)workspace_dev;
+    rbl::check_workspace(rbl::forward_workspace(*s), workspace_dev, workspace_bytes);
     rbl::DeviceScope scope(device);
     s->activation == RBL_ACT_GELU ? rbl::forward_by_type<RBL_ACT_GELU>(s->dtype, a, (hipStream_t)stream)
                                   : rbl::forward_by_type<RBL_ACT_NONE>(s->dtype, a, (hipStream_t)stream);
