@@ -6,9 +6,7 @@
 // and, with g = dy (GELU: g = dy (Phi(z) + z phi(z)), phi the density):
 //     db = sum_rows g     dw = sum_rows g h     dx = r (g w - sum(g w) / n - h sum(g w h) / n)
 //
-// Backward, simple form: a workgroup to a row, which it walks twice (the row stays in the caches); the parameters' gradients by
-// a second kernel that walks columns.  h is computed again from x and the two statistics of the row, so nothing else is kept
-// between the passes.
+// h is computed again from x and the two statistics of the row, so nothing else is kept between the passes.
 #include "train_kernels.h"
 
 namespace rbl {
@@ -60,7 +58,8 @@ struct NormArgs {
   void *y, *dx, *dw, *db;
   float* stats;    // [rows][2]: mean, 1 / sqrt(variance + eps)
   int64_t rows, x_stride, dy_stride;
-  float* partial;  // workspace
+  float* partial;   // workspace: statistics of chunks (forward), sums of the parameters' gradients (backward)
+  float* row_sums;  // workspace: chunks' sums of g w and g w h
   int cols;
   int chunks;     // of a row that is longer than a workgroup's registers
   int param_f32;  // the parameters' type: f32, or the rows' type
@@ -68,31 +67,11 @@ struct NormArgs {
 };
 
 template <class T>
-__device__ __forceinline__ float param(const NormArgs& a, const void* p, int col, float missing) {
-  if (!p) return missing;
-  return a.param_f32 ? ((const float*)p)[col] : (float)((const T*)p)[col];
-}
-template <class T>
 __device__ __forceinline__ void put_param(const NormArgs& a, void* p, int col, float v) {
   if (a.param_f32)
     ((float*)p)[col] = v;
   else
     ((T*)p)[col] = (T)v;
-}
-
-// Sums of two numbers over the workgroup, the same bits in every thread.
-__device__ __forceinline__ void sum_block(float& p, float& q, float (*slots)[2]) {
-  const int wave = threadIdx.x / 64;
-  p = sum64(p);
-  q = sum64(q);
-  __syncthreads();
-  if (threadIdx.x % 64 == 0) {
-    slots[wave][0] = p;
-    slots[wave][1] = q;
-  }
-  __syncthreads();
-  p = (slots[0][0] + slots[1][0]) + (slots[2][0] + slots[3][0]);
-  q = (slots[0][1] + slots[1][1]) + (slots[2][1] + slots[3][1]);
 }
 
 // V consecutive elements in one access: 16 bytes, at the alignment of an element (the memory pipe takes any).
@@ -336,58 +315,308 @@ __global__ __launch_bounds__(kThreads) void layer_norm_chunk_forward_kernel(Norm
   }
 }
 
-template <class T, int ACT>
-__global__ __launch_bounds__(kThreads) void layer_norm_dx_kernel(NormArgs a) {
-  __shared__ float slots[kThreads / 64][2];
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const T* x = (const T*)a.x + row * a.x_stride;
-    const T* dy = (const T*)a.dy + row * a.dy_stride;
-    T* dx = (T*)a.dx + row * a.cols;
-    const float mean = a.stats[2 * row], r = a.stats[2 * row + 1];
+// Workgroup size of the backward kernel: rows of up to 64 threads share a workgroup of eight wavefronts, so that fewer
+// partial sums of the parameters' gradients leave it.
+template <int TPR>
+constexpr int backward_threads() { return TPR <= 64 ? 512 : TPR; }
+
+// Writes what a thread has summed up over rows for its V columns: the owned ones alone.
+template <int V, bool EVEN>
+__device__ __forceinline__ void put_sums(float* out, const float (&v)[V], int skip) {
+  if (EVEN || skip == 0) {
+    typename Pack<float, V>::type p;
+#pragma unroll
+    for (int i = 0; i < V; ++i) p[i] = v[i];
+    *(typename Pack<float, V>::type*)out = p;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i >= skip) out[i] = v[i];
+  }
+}
+
+// Backward, a row in the registers of TPR threads: x and dy are read once, dx is written, and (SUMS) g h and g are summed up over
+// the rows of the workgroup, in registers; the workgroups' sums are joined by layer_norm_sums_kernel.
+template <class T, int V, int TPR, int K, bool EVEN, int ACT, bool SUMS>
+__global__ __launch_bounds__(backward_threads<TPR>()) void layer_norm_backward_kernel(NormArgs a) {
+  constexpr int NT = backward_threads<TPR>(), RPB = NT / TPR;
+  typedef typename Pack<T, V>::type vec;
+  __shared__ float slots[TPR > 64 ? 4 * TPR / 64 : 1];
+  __shared__ float joined[SUMS && TPR <= 64 ? 2 * TPR * K * V : 1];
+  int turn = 0;
+  const int t = threadIdx.x % TPR;
+  Place<V, TPR, EVEN> at[K];
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  constexpr bool KEEP = K * V <= 16;
+  float w[K][V], b[K][V], dw[K][V], db[K][V];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    at[k] = Place<V, TPR, EVEN>(t, k, a.cols);
+    if (KEEP) {
+      load_params<T, V>(a, a.w, at[k].col, 1.0f, w[k]);
+      if (ACT != RBL_ACT_NONE) load_params<T, V>(a, a.b, at[k].col, 0.0f, b[k]);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0;
+  }
+  if (row < a.rows) {
+    vec next_x[K], next_dy[K];
+    float2 next_s = *(const float2*)(a.stats + 2 * row);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      next_x[k] = *(const vec*)((const T*)a.x + row * a.x_stride + at[k].col);
+      next_dy[k] = *(const vec*)((const T*)a.dy + row * a.dy_stride + at[k].col);
+    }
+    for (; row < a.rows; row += step) {
+      const float mean = next_s.x, r = next_s.y;
+      float h[K][V], g[K][V];
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          h[k][i] = ((float)next_x[k][i] - mean) * r;
+          g[k][i] = at[k].owns(i) ? (float)next_dy[k][i] : 0.0f;
+        }
+      const int64_t ahead = row + step < a.rows ? row + step : row;
+      next_s = *(const float2*)(a.stats + 2 * ahead);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        next_x[k] = *(const vec*)((const T*)a.x + ahead * a.x_stride + at[k].col);
+        next_dy[k] = *(const vec*)((const T*)a.dy + ahead * a.dy_stride + at[k].col);
+      }
+      float s[2] = {0, 0};
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (!KEEP) {
+          load_params<T, V>(a, a.w, at[k].col, 1.0f, w[k]);
+          if (ACT != RBL_ACT_NONE) load_params<T, V>(a, a.b, at[k].col, 0.0f, b[k]);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          if (ACT != RBL_ACT_NONE) g[k][i] *= activate_slope<ACT>(__builtin_fmaf(h[k][i], w[k][i], b[k][i]));
+          if (SUMS) {
+            dw[k][i] = __builtin_fmaf(g[k][i], h[k][i], dw[k][i]);
+            db[k][i] += g[k][i];
+          }
+          g[k][i] *= w[k][i];
+          s[0] += g[k][i];
+          s[1] = __builtin_fmaf(g[k][i], h[k][i], s[1]);
+        }
+      }
+      if (a.dx) {
+        sum_group<TPR>(s, slots, turn);
+        const float p = s[0] / (float)a.cols, q = s[1] / (float)a.cols;
+        T* dx = (T*)a.dx + row * a.cols;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          vec out;
+#pragma unroll
+          for (int i = 0; i < V; ++i) out[i] = (T)(r * (g[k][i] - __builtin_fmaf(h[k][i], q, p)));
+          // a moved-back vector has no gradients for what its neighbour owns: it writes its own elements alone
+          if (EVEN || at[k].skip == 0) {
+            *(vec*)(dx + at[k].col) = out;
+          } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+              if (at[k].owns(i)) dx[at[k].col + i] = out[i];
+          }
+        }
+      }
+    }
+  }
+  if constexpr (SUMS) {
+    const int64_t width = (a.cols + 3) / 4 * 4;
+    float* out = a.partial + blockIdx.x * 2 * width;
+    if constexpr (TPR > 64) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        put_sums<V, EVEN>(out + at[k].col, dw[k], at[k].skip);
+        put_sums<V, EVEN>(out + width + at[k].col, db[k], at[k].skip);
+      }
+    } else {
+      // the groups add their sums up one after the other
+      constexpr int GROUPS = NT / 64;
+      if (TPR == 16) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          dw[0][i] += __shfl_xor(dw[0][i], 16);
+          dw[0][i] += __shfl_xor(dw[0][i], 32);
+          db[0][i] += __shfl_xor(db[0][i], 16);
+          db[0][i] += __shfl_xor(db[0][i], 32);
+        }
+      }
+      for (int group = 0; group < GROUPS; ++group) {
+        if ((int)threadIdx.x / 64 == group && (TPR == 64 || threadIdx.x % 64 < 16)) {
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              // element i of vector v at [i][v]: consecutive lanes in consecutive banks
+              float* p = joined + (k * V + i) * TPR + t;
+              if (group == 0) {
+                p[0] = dw[k][i];
+                p[TPR * K * V] = db[k][i];
+              } else {
+                p[0] += dw[k][i];
+                p[TPR * K * V] += db[k][i];
+              }
+            }
+        }
+        lds_barrier();
+      }
+      for (int j = threadIdx.x; j < 2 * TPR * K; j += NT) {
+        const int which = j / (TPR * K), v = j % (TPR * K), k = v / TPR;
+        const Place<V, TPR, EVEN> place(v % TPR, k, a.cols);
+        float sum[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] = joined[which * TPR * K * V + (k * V + i) * TPR + v % TPR];
+        put_sums<V, EVEN>(out + which * width + place.col, sum, place.skip);
+      }
+    }
+  }
+}
+
+// The parameters' gradients from `count` rows of partial sums, each [2][width]: 64 columns to a workgroup, 64 threads down the
+// rows, in an order that depends on the counts alone.
+constexpr int kSumsThreads = 1024;
+template <class T>
+__global__ __launch_bounds__(kSumsThreads) void layer_norm_sums_kernel(NormArgs a, int count) {
+  __shared__ float part[kSumsThreads / 64][64];
+  const int width = (a.cols + 3) / 4 * 4;
+  const int quad = threadIdx.x % 16, slice = threadIdx.x / 16;
+  const int64_t col = (int64_t)blockIdx.x * 64 + quad * 4;
+  typedef Pack<float, 4>::type vec;
+  float s[4] = {0, 0, 0, 0};
+  if (col < 2 * (int64_t)width) {
+#pragma unroll 4
+    for (int g = slice; g < count; g += kSumsThreads / 16) {
+      const vec v = *(const vec*)(a.partial + (int64_t)g * 2 * width + col);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] += v[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s[i] += __shfl_xor(s[i], 16);
+    s[i] += __shfl_xor(s[i], 32);
+    if (threadIdx.x % 64 < 16) part[threadIdx.x / 64][quad * 4 + i] = s[i];
+  }
+  lds_barrier();
+  const int64_t mine = (int64_t)blockIdx.x * 64 + threadIdx.x;
+  if (threadIdx.x < 64 && mine < 2 * (int64_t)width) {
+    float v = part[0][threadIdx.x];
+#pragma unroll
+    for (int k = 1; k < kSumsThreads / 64; ++k) v += part[k][threadIdx.x];
+    const bool second = mine >= width;
+    const int c = (int)(mine - (second ? width : 0));
+    if (c < a.cols) {
+      if (second && a.db) put_param<T>(a, a.db, c, v);
+      if (!second && a.dw) put_param<T>(a, a.dw, c, v);
+    }
+  }
+}
+
+// Longer rows, in chunks: first the chunks' shares of sum(g w) and sum(g w h) ...
+template <class T, int V, int ACT>
+__global__ __launch_bounds__(kThreads) void layer_norm_chunk_backward_sums_kernel(NormArgs a) {
+  typedef typename Pack<T, V>::type vec;
+  __shared__ float slots[4 * kThreads / 64];
+  int turn = 0;
+  for (int64_t item = blockIdx.x; item < a.rows * a.chunks; item += gridDim.x) {
+    const int64_t row = item / a.chunks;
+    const int begin = (int)(item - row * a.chunks) * chunk_cols<V>();
+    const int cols = min(a.cols - begin, chunk_cols<V>());
+    const T *x = (const T*)a.x + row * a.x_stride + begin, *dy = (const T*)a.dy + row * a.dy_stride + begin;
+    const float2 st = *(const float2*)(a.stats + 2 * row);
+    float s[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < kChunkK; ++k) {
+      const int at = (threadIdx.x + k * kThreads) * V, col = at + V <= cols ? at : cols - V;
+      const vec xs = *(const vec*)(x + col), ds = *(const vec*)(dy + col);
+      float w[V], b[V];
+      load_params<T, V>(a, a.w, begin + col, 1.0f, w);
+      if (ACT != RBL_ACT_NONE) load_params<T, V>(a, a.b, begin + col, 0.0f, b);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float h = ((float)xs[i] - st.x) * st.y;
+        float g = i >= at - col ? (float)ds[i] : 0.0f;
+        if (ACT != RBL_ACT_NONE) g *= activate_slope<ACT>(__builtin_fmaf(h, w[i], b[i]));
+        g *= w[i];
+        s[0] += g;
+        s[1] = __builtin_fmaf(g, h, s[1]);
+      }
+    }
+    sum_group<kThreads>(s, slots, turn);
+    if (threadIdx.x == 0) *(float2*)(a.row_sums + 2 * item) = make_float2(s[0], s[1]);
+  }
+}
+
+// ... then dx, and the parameters' gradients summed up over every `slices`-th row of a chunk
+template <class T, int V, int ACT, bool SUMS>
+__global__ __launch_bounds__(kThreads) void layer_norm_chunk_backward_kernel(NormArgs a, int slices) {
+  typedef typename Pack<T, V>::type vec;
+  const int chunk = blockIdx.x % a.chunks, slice = blockIdx.x / a.chunks;
+  const int begin = chunk * chunk_cols<V>(), cols = min(a.cols - begin, chunk_cols<V>());
+  int col[kChunkK], skip[kChunkK];
+  float dw[kChunkK][V], db[kChunkK][V];
+#pragma unroll
+  for (int k = 0; k < kChunkK; ++k) {
+    const int at = (threadIdx.x + k * kThreads) * V;
+    col[k] = begin + (at + V <= cols ? at : cols - V);
+    skip[k] = begin + at - col[k];
+#pragma unroll
+    for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0;
+  }
+  for (int64_t row = slice; row < a.rows; row += slices) {
+    vec xs[kChunkK], ds[kChunkK];
+#pragma unroll
+    for (int k = 0; k < kChunkK; ++k) {
+      xs[k] = *(const vec*)((const T*)a.x + row * a.x_stride + col[k]);
+      ds[k] = *(const vec*)((const T*)a.dy + row * a.dy_stride + col[k]);
+    }
+    const float2 st = *(const float2*)(a.stats + 2 * row);
     float p = 0, q = 0;
-    for (int c = threadIdx.x; c < a.cols; c += kThreads) {
-      const float h = ((float)x[c] - mean) * r, w = param<T>(a, a.w, c, 1.0f);
-      const float gw = (float)dy[c] * activate_slope<ACT>(__builtin_fmaf(h, w, param<T>(a, a.b, c, 0.0f))) * w;
-      p += gw;
-      q = __builtin_fmaf(gw, h, q);
+    if (a.dx) {
+      const float2* s = (const float2*)a.row_sums + row * a.chunks;
+      for (int c = threadIdx.x % 64; c < a.chunks; c += 64) {
+        p += s[c].x;
+        q += s[c].y;
+      }
+      p = sum64(p) / (float)a.cols;
+      q = sum64(q) / (float)a.cols;
     }
-    sum_block(p, q, slots);
-    p /= a.cols;
-    q /= a.cols;
-    for (int c = threadIdx.x; c < a.cols; c += kThreads) {
-      const float h = ((float)x[c] - mean) * r, w = param<T>(a, a.w, c, 1.0f);
-      const float gw = (float)dy[c] * activate_slope<ACT>(__builtin_fmaf(h, w, param<T>(a, a.b, c, 0.0f))) * w;
-      dx[c] = (T)(r * (gw - p - h * q));
+    T* dx = (T*)a.dx + row * a.cols;
+#pragma unroll
+    for (int k = 0; k < kChunkK; ++k) {
+      float w[V], b[V];
+      load_params<T, V>(a, a.w, col[k], 1.0f, w);
+      if (ACT != RBL_ACT_NONE) load_params<T, V>(a, a.b, col[k], 0.0f, b);
+      vec out;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float h = ((float)xs[k][i] - st.x) * st.y;
+        float g = (float)ds[k][i];
+        if (ACT != RBL_ACT_NONE) g *= activate_slope<ACT>(__builtin_fmaf(h, w[i], b[i]));
+        if (SUMS) {
+          dw[k][i] = __builtin_fmaf(g, h, dw[k][i]);
+          db[k][i] += g;
+        }
+        out[i] = (T)(st.y * (g * w[i] - __builtin_fmaf(h, q, p)));
+      }
+      if (a.dx && skip[k] < V) *(vec*)(dx + col[k]) = out;
+    }
+  }
+  if constexpr (SUMS) {
+    const int64_t width = (a.cols + 3) / 4 * 4;
+    float* out = a.partial + slice * 2 * width;
+#pragma unroll
+    for (int k = 0; k < kChunkK; ++k) {
+      put_sums<V, false>(out + col[k], dw[k], skip[k]);
+      put_sums<V, false>(out + width + col[k], db[k], skip[k]);
     }
   }
 }
-
-// 64 columns x 4 row threads to a workgroup, over all rows.
-template <class T, int ACT>
-__global__ __launch_bounds__(kThreads) void layer_norm_dparam_kernel(NormArgs a) {
-  __shared__ float part[2][4][64];
-  const int lane = threadIdx.x % 64, slice = threadIdx.x / 64;
-  const int c = blockIdx.x * 64 + lane;
-  float dw = 0, db = 0;
-  if (c < a.cols) {
-    const float w = param<T>(a, a.w, c, 1.0f), b = param<T>(a, a.b, c, 0.0f);
-    for (int64_t row = slice; row < a.rows; row += 4) {
-      const float h = ((float)((const T*)a.x)[row * a.x_stride + c] - a.stats[2 * row]) * a.stats[2 * row + 1];
-      const float g = (float)((const T*)a.dy)[row * a.dy_stride + c] * activate_slope<ACT>(__builtin_fmaf(h, w, b));
-      dw = __builtin_fmaf(g, h, dw);
-      db += g;
-    }
-  }
-  part[0][slice][lane] = dw;
-  part[1][slice][lane] = db;
-  __syncthreads();
-  if (slice == 0 && c < a.cols) {
-    if (a.dw) put_param<T>(a, a.dw, c, (part[0][0][lane] + part[0][1][lane]) + (part[0][2][lane] + part[0][3][lane]));
-    if (a.db) put_param<T>(a, a.db, c, (part[1][0][lane] + part[1][1][lane]) + (part[1][2][lane] + part[1][3][lane]));
-  }
-}
-
-unsigned row_grid(int64_t rows) { return (unsigned)(rows < 16384 ? rows : 16384); }
 
 constexpr int kCus = 256;
 
@@ -402,8 +631,8 @@ void forward_rows(NormArgs a, hipStream_t st) {
   launch(kernel, (unsigned)(need < most ? need : most), NT, args, st);
 }
 
-// The widest row that a workgroup holds in its registers, in vectors
-constexpr int kMostVectors = 4096;
+// The widest rows that a workgroup's registers hold, forward
+constexpr int kForwardCols = 16384;
 
 template <class T>
 int chunk_count(int cols) {
@@ -420,11 +649,19 @@ void run_forward(NormArgs a, hipStream_t st) {
   if (vectors <= 16) return forward_rows<T, V, 16, 1, ACT>(a, st);
   if (vectors <= 64) return forward_rows<T, V, 64, 1, ACT>(a, st);
   if (vectors <= 128) return forward_rows<T, V, 64, 2, ACT>(a, st);
-  if (vectors <= 256) return forward_rows<T, V, 64, 4, ACT>(a, st);
-  if (vectors <= 512) return forward_rows<T, V, 256, 2, ACT>(a, st);
-  if (vectors <= 1024) return forward_rows<T, V, 256, 4, ACT>(a, st);
-  if (vectors <= 2048) return forward_rows<T, V, 1024, 2, ACT>(a, st);
-  if (vectors <= kMostVectors) return forward_rows<T, V, 1024, 4, ACT>(a, st);
+  // up to 16 elements to a thread: more do not fit into the registers without spilling
+  if constexpr (V == 4) {
+    if (vectors <= 256) return forward_rows<T, V, 64, 4, ACT>(a, st);
+    if (vectors <= 512) return forward_rows<T, V, 256, 2, ACT>(a, st);
+    if (vectors <= 1024) return forward_rows<T, V, 256, 4, ACT>(a, st);
+    if (vectors <= 2048) return forward_rows<T, V, 1024, 2, ACT>(a, st);
+    if (vectors <= 4096) return forward_rows<T, V, 1024, 4, ACT>(a, st);
+  } else {
+    if (vectors <= 256) return forward_rows<T, V, 256, 1, ACT>(a, st);
+    if (vectors <= 512) return forward_rows<T, V, 256, 2, ACT>(a, st);
+    if (vectors <= 1024) return forward_rows<T, V, 1024, 1, ACT>(a, st);
+    if (vectors <= 2048) return forward_rows<T, V, 1024, 2, ACT>(a, st);
+  }
   a.chunks = chunk_count<T>(a.cols);
   const int64_t items = a.rows * a.chunks;
   const unsigned grid = (unsigned)(items < 1 << 20 ? items : 1 << 20);
@@ -432,12 +669,82 @@ void run_forward(NormArgs a, hipStream_t st) {
   launch((const void*)layer_norm_chunk_statistics_kernel<T, V>, grid, kThreads, args, st);
   launch((const void*)layer_norm_chunk_forward_kernel<T, V, ACT>, grid, kThreads, args, st);
 }
-template <class T, int ACT>
-void run_backward(NormArgs a, hipStream_t st) {
+// Workgroups of the backward kernels, i.e. rows of partial sums
+struct BackwardPlan {
+  int vectors, tpr, k;  // tpr 0: chunks
+  int chunks;
+  int64_t groups;
+};
+
+BackwardPlan backward_plan(const rbl_layer_norm_shape& s) {
+  const int v = s.dtype == RBL_F32 ? 4 : 8;
+  BackwardPlan p{};
+  p.vectors = (int)((s.cols + v - 1) / v);
+  if (s.cols < v || p.vectors <= 16) p.tpr = 16, p.k = 1;
+  else if (p.vectors <= 64) p.tpr = 64, p.k = 1;
+  else if (p.vectors <= 128) p.tpr = 64, p.k = 2;
+  else if (v == 4 && p.vectors <= 256) p.tpr = 64, p.k = 4;
+  else if (p.vectors <= 256) p.tpr = 256, p.k = 1;
+  else if (p.vectors <= 512) p.tpr = 256, p.k = 2;
+  else if (p.vectors <= 1024) p.tpr = 512, p.k = 2;
+  else if (v == 4 && p.vectors <= 2048) p.tpr = 512, p.k = 4;
+  if (p.tpr) {
+    const int nt = p.tpr <= 64 ? 512 : p.tpr;
+    const int64_t need = (s.rows * p.tpr + nt - 1) / nt, most = (int64_t)kCus * (1024 / nt);
+    p.groups = need < most ? need : most;
+  } else {
+    p.chunks = (int)((s.cols + kThreads * kChunkK * v - 1) / (kThreads * kChunkK * v));
+    const int64_t most = (kCus + p.chunks - 1) / p.chunks;
+    p.groups = s.rows < most ? s.rows : most;
+  }
+  return p;
+}
+
+template <class T, int V, int TPR, int K, int ACT>
+void backward_rows(NormArgs a, const BackwardPlan& p, bool sums, hipStream_t st) {
+  const bool even = a.cols == TPR * K * V;
+  const void* kernel = sums ? even ? (const void*)layer_norm_backward_kernel<T, V, TPR, K, true, ACT, true>
+                                   : (const void*)layer_norm_backward_kernel<T, V, TPR, K, false, ACT, true>
+                       : even ? (const void*)layer_norm_backward_kernel<T, V, TPR, K, true, ACT, false>
+                              : (const void*)layer_norm_backward_kernel<T, V, TPR, K, false, ACT, false>;
   void* args[] = {&a};
-  if (a.dx && a.rows > 0) launch((const void*)layer_norm_dx_kernel<T, ACT>, row_grid(a.rows), kThreads, args, st);
-  if (a.dw || a.db)
-    launch((const void*)layer_norm_dparam_kernel<T, ACT>, (unsigned)((a.cols + 63) / 64), kThreads, args, st);
+  launch(kernel, (unsigned)p.groups, backward_threads<TPR>(), args, st);
+}
+
+template <class T, int ACT>
+void run_backward(NormArgs a, const BackwardPlan& p, hipStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const bool sums = a.dw || a.db;
+  if (a.rows > 0 && (a.dx || sums)) {
+    if (a.cols < V) backward_rows<T, 1, 16, 1, ACT>(a, p, sums, st);
+    else if (p.tpr == 16) backward_rows<T, V, 16, 1, ACT>(a, p, sums, st);
+    else if (p.tpr == 64 && p.k == 1) backward_rows<T, V, 64, 1, ACT>(a, p, sums, st);
+    else if (p.tpr == 64 && p.k == 2) backward_rows<T, V, 64, 2, ACT>(a, p, sums, st);
+    else if (p.tpr == 64) { if constexpr (V == 4) backward_rows<T, V, 64, 4, ACT>(a, p, sums, st); }
+    else if (p.tpr == 256 && p.k == 1) { if constexpr (V == 8) backward_rows<T, V, 256, 1, ACT>(a, p, sums, st); }
+    else if (p.tpr == 256) backward_rows<T, V, 256, 2, ACT>(a, p, sums, st);
+    else if (p.tpr == 512 && p.k == 2) backward_rows<T, V, 512, 2, ACT>(a, p, sums, st);
+    else if (p.tpr == 512) { if constexpr (V == 4) backward_rows<T, V, 512, 4, ACT>(a, p, sums, st); }
+    else {
+      a.chunks = p.chunks;
+      const int64_t items = a.rows * a.chunks;
+      void* args[] = {&a};
+      if (a.dx)
+        launch((const void*)layer_norm_chunk_backward_sums_kernel<T, V, ACT>, (unsigned)(items < 1 << 20 ? items : 1 << 20),
+               kThreads, args, st);
+      int slices = (int)p.groups;
+      void* more[] = {&a, &slices};
+      launch(sums ? (const void*)layer_norm_chunk_backward_kernel<T, V, ACT, true>
+                  : (const void*)layer_norm_chunk_backward_kernel<T, V, ACT, false>,
+             (unsigned)(p.groups * p.chunks), kThreads, more, st);
+    }
+  }
+  if (sums) {
+    int count = (int)p.groups;
+    void* args[] = {&a, &count};
+    const int64_t width = (a.cols + 3) / 4 * 4;
+    launch((const void*)layer_norm_sums_kernel<T>, (unsigned)((2 * width + 63) / 64), kSumsThreads, args, st);
+  }
 }
 
 void check(const rbl_layer_norm_shape* s) {
@@ -455,9 +762,18 @@ void check(const rbl_layer_norm_shape* s) {
 
 int64_t forward_workspace(const rbl_layer_norm_shape& s) {
   const int size = s.dtype == RBL_F32 ? 4 : 2, v = 16 / size;
-  if (s.cols <= (int64_t)kMostVectors * v) return 0;
+  if (s.cols <= kForwardCols) return 0;
   const int64_t chunk = kThreads * kChunkK * v;
   return s.rows * ((s.cols + chunk - 1) / chunk) * 2 * (int64_t)sizeof(float);
+}
+
+// row_sums of the chunks, then the partial sums
+int64_t backward_row_sums(const rbl_layer_norm_shape& s, const BackwardPlan& p) {
+  return p.tpr ? 0 : s.rows * p.chunks * 2 * (int64_t)sizeof(float);
+}
+int64_t backward_workspace(const rbl_layer_norm_shape& s) {
+  const BackwardPlan p = backward_plan(s);
+  return (backward_row_sums(s, p) + 15) / 16 * 16 + p.groups * 2 * ((s.cols + 3) / 4 * 4) * (int64_t)sizeof(float);
 }
 
 void check_workspace(int64_t need, const void* workspace, int64_t bytes) {
@@ -483,10 +799,10 @@ void forward_by_type(int dtype, const NormArgs& a, hipStream_t st) {
   if (dtype == RBL_BF16) run_forward<__bf16, ACT>(a, st);
 }
 template <int ACT>
-void backward_by_type(int dtype, const NormArgs& a, hipStream_t st) {
-  if (dtype == RBL_F32) run_backward<float, ACT>(a, st);
-  if (dtype == RBL_F16) run_backward<_Float16, ACT>(a, st);
-  if (dtype == RBL_BF16) run_backward<__bf16, ACT>(a, st);
+void backward_by_type(int dtype, const NormArgs& a, const BackwardPlan& p, hipStream_t st) {
+  if (dtype == RBL_F32) run_backward<float, ACT>(a, p, st);
+  if (dtype == RBL_F16) run_backward<_Float16, ACT>(a, p, st);
+  if (dtype == RBL_BF16) run_backward<__bf16, ACT>(a, p, st);
 }
 
 }  // namespace
@@ -498,7 +814,7 @@ int64_t rbl_layer_norm_workspace(const rbl_layer_norm_shape* s, int backward) {
   int64_t bytes = -1;
   rbl::train_entry([&] {
     rbl::check(s);
-    bytes = backward ? 0 : rbl::forward_workspace(*s);
+    bytes = backward ? rbl::backward_workspace(*s) : rbl::forward_workspace(*s);
   });
   return bytes;
 }
@@ -538,9 +854,13 @@ int rbl_layer_norm_backward(int device, const rbl_layer_norm_shape* s, const voi
     a.dx = dx_dev;
     a.dw = dweight_dev;
     a.db = dbias_dev;
+    rbl::check_workspace(rbl::backward_workspace(*s), workspace_dev, workspace_bytes);
+    const rbl::BackwardPlan p = rbl::backward_plan(*s);
+    a.row_sums = (float*)workspace_dev;
+    a.partial = a.row_sums + (rbl::backward_row_sums(*s, p) + 15) / 16 * 4;
     rbl::DeviceScope scope(device);
-    s->activation == RBL_ACT_GELU ? rbl::backward_by_type<RBL_ACT_GELU>(s->dtype, a, (hipStream_t)stream)
-                                  : rbl::backward_by_type<RBL_ACT_NONE>(s->dtype, a, (hipStream_t)stream);
+    s->activation == RBL_ACT_GELU ? rbl::backward_by_type<RBL_ACT_GELU>(s->dtype, a, p, (hipStream_t)stream)
+                                  : rbl::backward_by_type<RBL_ACT_NONE>(s->dtype, a, p, (hipStream_t)stream);
   });
 }
 
