@@ -15,50 +15,56 @@ namespace rbl {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTableSize = 128;      // tensors per launch
+constexpr int kTableSize = 240;      // tensors per launch
 constexpr int64_t kChunkMin = 2048;  // elements
 constexpr int kChunksAim = 2048;     // workgroups that fill the chip: 8 to a CU
 
 struct GradTable {
   void* data[kTableSize];
-  int64_t numel[kTableSize];
   int first_chunk[kTableSize + 1];
-  int8_t dtype[kTableSize];
+  unsigned last[kTableSize];  // elements of the tensor's last chunk; its type in the upper two bits
 };
+constexpr int kTypeShift = 30;
 
 struct ClipArgs {
   double* sums;          // one per chunk
   const float* norm_in;  // the norm, where it is known already
   float* norm_out;
   double max_norm;
-  int64_t chunk;
-  int count;       // tensors in the table
-  int first;       // chunks before the table's first
-  int total;       // chunks of all tables
-  int norm;
+  int chunk;  // elements
+  int count;  // tensors in the table
+  int first;  // chunks before the table's first
+  int total;  // chunks of all tables
 };
+static_assert(sizeof(GradTable) + sizeof(ClipArgs) <= 4096, "kernel arguments");
 
-__device__ __forceinline__ double magnitude(float v, int norm) {
+// One element's share of the norm, and how shares are joined: the sum, or the maximum that keeps a NaN.
+template <int NORM>
+__device__ __forceinline__ void take(double& s, float v) {
   const double d = v;
-  return norm == RBL_NORM_2 ? d * d : __builtin_fabs(d);
+  if (NORM == RBL_NORM_2) s = __builtin_fma(d, d, s);
+  if (NORM == RBL_NORM_1) s += __builtin_fabs(d);
+  if (NORM == RBL_NORM_INF) s = (__builtin_fabs(d) > s || d != d) ? __builtin_fabs(d) : s;
 }
-// Sum, or the maximum that keeps a NaN
-__device__ __forceinline__ double join(double a, double b, int norm) {
-  if (norm != RBL_NORM_INF) return a + b;
+template <int NORM>
+__device__ __forceinline__ double join(double a, double b) {
+  if (NORM != RBL_NORM_INF) return a + b;
   return (b > a || b != b) ? b : a;
 }
 
-__device__ __forceinline__ double join_block(double v, int norm, double* slots) {
-  for (int d = 1; d < 64; d *= 2) v = join(v, __shfl_xor(v, d), norm);
+template <int NORM>
+__device__ __forceinline__ double join_block(double v, double* slots) {
+  for (int d = 1; d < 64; d *= 2) v = join<NORM>(v, __shfl_xor(v, d));
   if (threadIdx.x % 64 == 0) slots[threadIdx.x / 64] = v;
   __syncthreads();
-  return join(join(slots[0], slots[1], norm), join(slots[2], slots[3], norm), norm);
+  return join<NORM>(join<NORM>(slots[0], slots[1]), join<NORM>(slots[2], slots[3]));
 }
 
-// The chunk of this workgroup: which tensor, from where to where
+// A workgroup's chunk: its first element, how many, and their type
 struct Chunk {
-  int tensor;
-  int64_t begin, end;
+  void* data;
+  int64_t begin;
+  int count, type;
 };
 __device__ __forceinline__ Chunk chunk_of(const GradTable& t, const ClipArgs& a, int index) {
   int lo = 0, hi = a.count;  // first_chunk[lo] <= index < first_chunk[hi]
@@ -69,62 +75,136 @@ __device__ __forceinline__ Chunk chunk_of(const GradTable& t, const ClipArgs& a,
     else
       hi = mid;
   }
-  const int64_t begin = (index - t.first_chunk[lo]) * a.chunk, end = begin + a.chunk;
-  return {lo, begin, end < t.numel[lo] ? end : t.numel[lo]};
+  const unsigned last = t.last[lo];
+  const bool is_last = index + 1 == t.first_chunk[lo + 1];
+  return {t.data[lo], (int64_t)(index - t.first_chunk[lo]) * a.chunk,
+          is_last ? (int)(last & ((1u << kTypeShift) - 1)) : a.chunk, (int)(last >> kTypeShift)};
 }
 
+// 16 bytes in one access, at the alignment of an element
 template <class T>
-__device__ __forceinline__ double sum_chunk(const T* g, int64_t begin, int64_t end, int norm) {
-  double v = 0;
-  for (int64_t i = begin + threadIdx.x; i < end; i += kThreads) v = join(v, magnitude((float)g[i], norm), norm);
-  return v;
+struct Pack {
+  static constexpr int V = 16 / sizeof(T);
+  typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+};
+
+constexpr int kAhead = 4;  // loads in flight per thread
+
+template <class T, int NORM>
+__device__ __forceinline__ double sum_chunk(const T* g, int count) {
+  constexpr int V = Pack<T>::V, STEP = kThreads * V;
+  typedef typename Pack<T>::type vec;
+  double s[2] = {0, 0};
+  int i = threadIdx.x * V;
+  for (; i + (kAhead - 1) * STEP + V <= count; i += kAhead * STEP) {
+    vec v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) v[k] = *(const vec*)(g + i + k * STEP);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) take<NORM>(s[j % 2], (float)v[k][j]);
+  }
+  for (; i + V <= count; i += STEP) {
+    const vec v = *(const vec*)(g + i);
+#pragma unroll
+    for (int j = 0; j < V; ++j) take<NORM>(s[j % 2], (float)v[j]);
+  }
+  const int rest = count / V * V + (int)threadIdx.x;  // fewer than V elements behind the last whole vector
+  if (rest < count) take<NORM>(s[0], (float)g[rest]);
+  return join<NORM>(s[0], s[1]);
 }
 
+template <int NORM>
 __global__ __launch_bounds__(kThreads) void grad_sums_kernel(GradTable t, ClipArgs a) {
   __shared__ double slots[kThreads / 64];
   const Chunk k = chunk_of(t, a, blockIdx.x);
-  const void* p = t.data[k.tensor];
-  const int dtype = t.dtype[k.tensor];
-  double v = dtype == RBL_F32   ? sum_chunk((const float*)p, k.begin, k.end, a.norm)
-             : dtype == RBL_F16 ? sum_chunk((const _Float16*)p, k.begin, k.end, a.norm)
-                                : sum_chunk((const __bf16*)p, k.begin, k.end, a.norm);
-  v = join_block(v, a.norm, slots);
+  double v = k.type == RBL_F32   ? sum_chunk<float, NORM>((const float*)k.data + k.begin, k.count)
+             : k.type == RBL_F16 ? sum_chunk<_Float16, NORM>((const _Float16*)k.data + k.begin, k.count)
+                                 : sum_chunk<__bf16, NORM>((const __bf16*)k.data + k.begin, k.count);
+  v = join_block<NORM>(v, slots);
   if (threadIdx.x == 0) a.sums[a.first + blockIdx.x] = v;
 }
 
+template <int NORM>
 __device__ __forceinline__ double whole_norm(const ClipArgs& a, double* slots) {
   double v = 0;
-  for (int i = threadIdx.x; i < a.total; i += kThreads) v = join(v, a.sums[i], a.norm);
-  v = join_block(v, a.norm, slots);
-  return a.norm == RBL_NORM_2 ? __builtin_sqrt(v) : v;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < a.total; i += kThreads) v = join<NORM>(v, a.sums[i]);
+  v = join_block<NORM>(v, slots);
+  return NORM == RBL_NORM_2 ? __builtin_sqrt(v) : v;
 }
 
 template <class T>
-__device__ __forceinline__ void scale_chunk(T* g, int64_t begin, int64_t end, float c) {
-  for (int64_t i = begin + threadIdx.x; i < end; i += kThreads) g[i] = (T)((float)g[i] * c);
+__device__ __forceinline__ void scale_chunk(T* g, int count, float c) {
+  constexpr int V = Pack<T>::V, STEP = kThreads * V;
+  typedef typename Pack<T>::type vec;
+  int i = threadIdx.x * V;
+  for (; i + (kAhead - 1) * STEP + V <= count; i += kAhead * STEP) {
+    vec v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) v[k] = *(const vec*)(g + i + k * STEP);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[k][j] = (T)((float)v[k][j] * c);
+      *(vec*)(g + i + k * STEP) = v[k];
+    }
+  }
+  for (; i + V <= count; i += STEP) {
+    vec v = *(const vec*)(g + i);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = (T)((float)v[j] * c);
+    *(vec*)(g + i) = v;
+  }
+  const int rest = count / V * V + (int)threadIdx.x;
+  if (rest < count) g[rest] = (T)((float)g[rest] * c);
 }
 
+// NORM 0: the norm is there already
+template <int NORM>
 __global__ __launch_bounds__(kThreads) void grad_scale_kernel(GradTable t, ClipArgs a) {
   __shared__ double slots[kThreads / 64];
-  const double norm = a.norm_in ? (double)*a.norm_in : whole_norm(a, slots);
-  if (a.norm_out && a.first == 0 && blockIdx.x == 0 && threadIdx.x == 0) *a.norm_out = (float)norm;
+  double norm;
+  if constexpr (NORM == 0) {
+    norm = (double)*a.norm_in;
+  } else {
+    norm = whole_norm<NORM>(a, slots);
+    if (a.first == 0 && blockIdx.x == 0 && threadIdx.x == 0) *a.norm_out = (float)norm;
+  }
   const double c = a.max_norm / (norm + 1e-6);
   if (c >= 1.0) return;  // times 1: nothing changes
-  const Chunk k = chunk_of(t, a, blockIdx.x);
-  void* p = t.data[k.tensor];
-  const int dtype = t.dtype[k.tensor];
-  if (dtype == RBL_F32)
-    scale_chunk((float*)p, k.begin, k.end, (float)c);
-  else if (dtype == RBL_F16)
-    scale_chunk((_Float16*)p, k.begin, k.end, (float)c);
+  // from the last chunk to the first: what the sums read last is what the cache still has
+  const Chunk k = chunk_of(t, a, gridDim.x - 1 - blockIdx.x);
+  if (k.type == RBL_F32)
+    scale_chunk((float*)k.data + k.begin, k.count, (float)c);
+  else if (k.type == RBL_F16)
+    scale_chunk((_Float16*)k.data + k.begin, k.count, (float)c);
   else
-    scale_chunk((__bf16*)p, k.begin, k.end, (float)c);
+    scale_chunk((__bf16*)k.data + k.begin, k.count, (float)c);
 }
 
+template <int NORM>
 __global__ __launch_bounds__(kThreads) void grad_norm_kernel(ClipArgs a) {
   __shared__ double slots[kThreads / 64];
-  const double norm = whole_norm(a, slots);
+  const double norm = whole_norm<NORM>(a, slots);
   if (threadIdx.x == 0) *a.norm_out = (float)norm;
+}
+
+template <int NORM>
+struct Kernels {
+  static const void* sums() { return (const void*)grad_sums_kernel<NORM>; }
+  static const void* scale() { return (const void*)grad_scale_kernel<NORM>; }
+  static const void* norm() { return (const void*)grad_norm_kernel<NORM>; }
+};
+const void* sums_kernel(int norm) {
+  return norm == RBL_NORM_1 ? Kernels<RBL_NORM_1>::sums() : norm == RBL_NORM_2 ? Kernels<RBL_NORM_2>::sums() : Kernels<RBL_NORM_INF>::sums();
+}
+const void* scale_kernel(int norm) {
+  return norm == RBL_NORM_1 ? Kernels<RBL_NORM_1>::scale() : norm == RBL_NORM_2 ? Kernels<RBL_NORM_2>::scale() : Kernels<RBL_NORM_INF>::scale();
+}
+const void* norm_kernel(int norm) {
+  return norm == RBL_NORM_1 ? Kernels<RBL_NORM_1>::norm() : norm == RBL_NORM_2 ? Kernels<RBL_NORM_2>::norm() : Kernels<RBL_NORM_INF>::norm();
 }
 
 int64_t chunk_size(const rbl_grad* grads, int n) {
@@ -143,7 +223,7 @@ int64_t chunk_count(const rbl_grad* grads, int n, int64_t chunk) {
 void check(const rbl_grad* grads, int n) {
   if (n < 0) throw std::runtime_error("gradients: n is negative");
   if (n > 0 && !grads) throw std::runtime_error("gradients: the list is null");
-  int64_t room = (int64_t)1 << 60;
+  int64_t room = (int64_t)1 << 40;  // a chunk's length fits into 30 bits
   for (int i = 0; i < n; ++i) {
     if (grads[i].numel < 0 || grads[i].numel > room) throw std::runtime_error("gradients: numel is negative or too large");
     room -= grads[i].numel;
@@ -165,29 +245,41 @@ void check_bound(double max_norm) {
   if (!(max_norm >= 0)) throw std::runtime_error("gradients: max_norm must be a number >= 0");
 }
 
-// One launch of `kernel` for every table of tensors
-void for_tables(const void* kernel, const rbl_grad* grads, int n, ClipArgs a, hipStream_t st) {
-  GradTable t;
-  a.chunk = chunk_size(grads, n);
+// One launch of `kernel` for every table of tensors; `backwards`: the last table first
+void for_tables(const void* kernel, const rbl_grad* grads, int n, ClipArgs a, bool backwards, hipStream_t st) {
+  a.chunk = (int)chunk_size(grads, n);
   a.total = (int)chunk_count(grads, n, a.chunk);
-  a.first = 0;
-  for (int i = 0; i < n;) {
-    int count = 0, chunks = 0;
-    for (; i < n && count < kTableSize; ++i) {
+  GradTable t;
+  int from = 0, to = n, first = backwards ? a.total : 0;
+  while (from < to) {
+    // the next table: tensors [from, end), or backwards [end, to)
+    int end = backwards ? to : from, count = 0;
+    while (backwards ? end > from : end < to) {
+      if (count == kTableSize) break;
+      if (grads[backwards ? end - 1 : end].numel > 0) ++count;
+      end += backwards ? -1 : 1;
+    }
+    const int lo = backwards ? end : from, hi = backwards ? to : end;
+    int chunks = 0;
+    count = 0;
+    for (int i = lo; i < hi; ++i) {
       if (grads[i].numel == 0) continue;
+      const int64_t whole = (grads[i].numel + a.chunk - 1) / a.chunk;
       t.data[count] = grads[i].data_dev;
-      t.numel[count] = grads[i].numel;
-      t.dtype[count] = (int8_t)grads[i].dtype;
       t.first_chunk[count] = chunks;
-      chunks += (int)((grads[i].numel + a.chunk - 1) / a.chunk);
+      t.last[count] = (unsigned)(grads[i].numel - (whole - 1) * a.chunk) | (unsigned)grads[i].dtype << kTypeShift;
+      chunks += (int)whole;
       ++count;
     }
-    if (count == 0) break;
-    t.first_chunk[count] = chunks;
-    a.count = count;
-    void* args[] = {&t, &a};
-    launch(kernel, (unsigned)chunks, kThreads, args, st);
-    a.first += chunks;
+    if (count > 0) {
+      t.first_chunk[count] = chunks;
+      a.count = count;
+      a.first = backwards ? first - chunks : first;
+      void* args[] = {&t, &a};
+      launch(kernel, (unsigned)chunks, kThreads, args, st);
+      first += backwards ? -chunks : chunks;
+    }
+    (backwards ? to : from) = end;
   }
 }
 
@@ -216,11 +308,10 @@ int rbl_grad_norm(int device, const rbl_grad* grads, int n, int norm, float* nor
     rbl::ClipArgs a{};
     a.sums = (double*)workspace_dev;
     a.norm_out = norm_dev;
-    a.norm = norm;
-    rbl::for_tables((const void*)rbl::grad_sums_kernel, grads, n, a, (hipStream_t)stream);
+    rbl::for_tables(rbl::sums_kernel(norm), grads, n, a, false, (hipStream_t)stream);
     a.total = (int)rbl::chunk_count(grads, n, rbl::chunk_size(grads, n));
     void* args[] = {&a};
-    rbl::launch((const void*)rbl::grad_norm_kernel, 1, rbl::kThreads, args, (hipStream_t)stream);
+    rbl::launch(rbl::norm_kernel(norm), 1, rbl::kThreads, args, (hipStream_t)stream);
   });
 }
 
@@ -236,14 +327,13 @@ int rbl_grad_clip(int device, const rbl_grad* grads, int n, int norm, double max
     rbl::ClipArgs a{};
     a.sums = (double*)workspace_dev;
     a.norm_out = norm_dev;
-    a.norm = norm;
     a.max_norm = max_norm;
-    rbl::for_tables((const void*)rbl::grad_sums_kernel, grads, n, a, (hipStream_t)stream);
+    rbl::for_tables(rbl::sums_kernel(norm), grads, n, a, false, (hipStream_t)stream);
     if (rbl::chunk_count(grads, n, rbl::chunk_size(grads, n)) == 0) {  // nothing to scale: the norm of nothing
       void* args[] = {&a};
-      rbl::launch((const void*)rbl::grad_norm_kernel, 1, rbl::kThreads, args, (hipStream_t)stream);
+      rbl::launch(rbl::norm_kernel(norm), 1, rbl::kThreads, args, (hipStream_t)stream);
     }
-    rbl::for_tables((const void*)rbl::grad_scale_kernel, grads, n, a, (hipStream_t)stream);
+    rbl::for_tables(rbl::scale_kernel(norm), grads, n, a, true, (hipStream_t)stream);
   });
 }
 
@@ -256,7 +346,7 @@ int rbl_grad_scale(int device, const rbl_grad* grads, int n, double max_norm, co
     rbl::ClipArgs a{};
     a.norm_in = norm_dev;
     a.max_norm = max_norm;
-    rbl::for_tables((const void*)rbl::grad_scale_kernel, grads, n, a, (hipStream_t)stream);
+    rbl::for_tables((const void*)rbl::grad_scale_kernel<0>, grads, n, a, true, (hipStream_t)stream);
   });
 }
 
