@@ -93,8 +93,21 @@ struct Place {
     skip = EVEN ? 0 : at - col;
   }
   __device__ __forceinline__ bool owns(int i) const { return EVEN || i >= skip; }
-  __device__ __forceinline__ bool any() const { return EVEN || skip < V; }
 };
+
+// Stores the elements that a thread owns.  A moved-back vector stores its own alone: what it has computed for its neighbour's
+// may differ in the last bit, since the compiler need not round the same way at another place of the vector.
+template <bool EVEN, class T, class VEC>
+__device__ __forceinline__ void put_row(T* out, const VEC& v, int skip) {
+  constexpr int V = sizeof(VEC) / sizeof(T);
+  if (EVEN || skip == 0) {
+    *(VEC*)out = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i >= skip) out[i] = v[i];
+  }
+}
 
 template <class T, int V>
 __device__ __forceinline__ void load_params(const NormArgs& a, const void* p, int col, float missing, float (&out)[V]) {
@@ -212,8 +225,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_forward_kern
       vec out;
 #pragma unroll
       for (int i = 0; i < V; ++i) out[i] = (T)activate<ACT>(__builtin_fmaf((x[k][i] - mean) * r, w[k][i], b[k][i]));
-      // a moved-back vector writes again what its neighbour writes, the same values
-      if (at[k].any()) *(vec*)(y + at[k].col) = out;
+      put_row<EVEN>(y + at[k].col, out, at[k].skip);
     }
     if (a.stats && t == 0) *(float2*)(a.stats + 2 * row) = make_float2(mean, r);
   }
@@ -309,7 +321,7 @@ __global__ __launch_bounds__(kThreads) void layer_norm_chunk_forward_kernel(Norm
       vec out;
 #pragma unroll
       for (int i = 0; i < V; ++i) out[i] = (T)activate<ACT>(__builtin_fmaf(((float)p[k][i] - mean) * r, w[i], b[i]));
-      if ((threadIdx.x + k * kThreads) * V - col[k] < V) *(vec*)(y + col[k]) = out;
+      put_row<false>(y + col[k], out, (threadIdx.x + k * kThreads) * V - col[k]);
     }
     if (a.stats && begin == 0 && threadIdx.x == 0) *(float2*)(a.stats + 2 * row) = make_float2(mean, r);
   }
@@ -413,14 +425,7 @@ __global__ __launch_bounds__(backward_threads<TPR>()) void layer_norm_backward_k
           vec out;
 #pragma unroll
           for (int i = 0; i < V; ++i) out[i] = (T)(r * (g[k][i] - __builtin_fmaf(h[k][i], q, p)));
-          // a moved-back vector has no gradients for what its neighbour owns: it writes its own elements alone
-          if (EVEN || at[k].skip == 0) {
-            *(vec*)(dx + at[k].col) = out;
-          } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-              if (at[k].owns(i)) dx[at[k].col + i] = out[i];
-          }
+          put_row<EVEN>(dx + at[k].col, out, at[k].skip);
         }
       }
     }
@@ -604,7 +609,7 @@ __global__ __launch_bounds__(kThreads) void layer_norm_chunk_backward_kernel(Nor
         }
         out[i] = (T)(st.y * (g * w[i] - __builtin_fmaf(h, q, p)));
       }
-      if (a.dx && skip[k] < V) *(vec*)(dx + col[k]) = out;
+      if (a.dx) put_row<false>(dx + col[k], out, skip[k]);
     }
   }
   if constexpr (SUMS) {

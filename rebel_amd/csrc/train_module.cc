@@ -6,10 +6,13 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 
 #include <algorithm>
 #include <cmath>
+#include <mutex>
 #include <optional>
 #include <stdexcept>
 #include <vector>
@@ -119,60 +122,77 @@ void refuse_foreign_accumulator(const Tensor& t) {
               "capturing (or make it on the capturing stream)");
 }
 
-class LayerNormFn : public torch::autograd::Function<LayerNormFn> {
+// The backward pass of one layer_norm call.  Edges: x, weight, bias (empty where one was not given).
+class LayerNormBackward : public torch::autograd::Node {
  public:
-  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x_in, const OptTensor& w_in, const OptTensor& b_in,
-                        double eps, int64_t activation) {
-    const Tensor x = with_rows(x_in), w = w_in ? w_in->contiguous() : Tensor(), b = b_in ? b_in->contiguous() : Tensor();
-    Tensor stats;
-    Tensor y = ::forward(x, w, b, eps, activation, &stats);
+  LayerNormBackward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& stats, double eps, int64_t activation,
+                    at::ScalarType param_type)
+      : x_(x, false), stats_(stats), eps_(eps), activation_(activation), param_type_(param_type) {
+    if (w.defined()) w_ = torch::autograd::SavedVariable(w, false);
     // the bias comes back only where the activation's slope depends on it
-    ctx->save_for_backward({x, w, activation == RBL_ACT_NONE ? Tensor() : b, stats});
-    ctx->saved_data["eps"] = eps;
-    ctx->saved_data["activation"] = activation;
-    ctx->saved_data["given"] = (int64_t)(w.defined() + 2 * b.defined());
-    ctx->saved_data["param_type"] =
-        (int64_t)(w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : at::kFloat);
-    return y;
+    if (b.defined() && activation != RBL_ACT_NONE) b_ = torch::autograd::SavedVariable(b, false);
   }
 
-  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     if (at::GradMode::is_enabled())
       throw std::runtime_error("layer_norm: its gradient has no gradient of its own (create_graph)");
-    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
-    const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &stats = saved[3];
+    std::lock_guard<std::mutex> lock(mutex_);
+    torch::autograd::variable_list out(3);
+    if (!grads[0].defined()) return out;
+    at::AutoDispatchBelowADInplaceOrView plain;
+    const Tensor x = x_.unpack(), w = w_.unpack(), b = b_.unpack();
     c10::DeviceGuard guard(x.device());
     const Tensor dy = with_rows(grads[0]);
-    rbl_layer_norm_shape s = shape_of(x, w, b, ctx->saved_data["eps"].toDouble(), ctx->saved_data["activation"].toInt());
-    const auto param_type = (at::ScalarType)ctx->saved_data["param_type"].toInt();
-    s.param_dtype = element_type(param_type);
+    rbl_layer_norm_shape s = shape_of(x, w, b, eps_, activation_);
+    s.param_dtype = element_type(param_type_);
     s.x_stride = row_stride(x);
     s.dy_stride = row_stride(dy);
-    Tensor dx, dw, db;
-    if (ctx->needs_input_grad(0)) dx = at::empty(x.sizes(), x.options());
-    // the edges count only the parameters that were given
-    const int64_t given = ctx->saved_data["given"].toInt();
-    const bool has_w = given & 1, has_b = given & 2;
-    if (has_w && ctx->needs_input_grad(1)) dw = at::empty({s.cols}, x.options().dtype(param_type));
-    if (has_b && ctx->needs_input_grad(1 + has_w)) db = at::empty({s.cols}, x.options().dtype(param_type));
-    Tensor space = workspace(x, rbl_layer_norm_workspace(&s, 1));
-    check(rbl_layer_norm_backward(x.get_device(), &s, data(dy), data(x), data(w), data(b), stats.data_ptr<float>(), data(dx),
-                                  data(dw), data(db), data(space), space.defined() ? space.numel() : 0, stream_of(x)));
-    return {dx, dw, db, Tensor(), Tensor()};
+    if (task_should_compute_output(0)) out[0] = at::empty(x.sizes(), x.options());
+    for (int i = 1; i < 3; ++i)
+      if (task_should_compute_output(i)) out[i] = at::empty({s.cols}, x.options().dtype(param_type_));
+    const Tensor space = workspace(x, rbl_layer_norm_workspace(&s, 1));
+    check(rbl_layer_norm_backward(x.get_device(), &s, data(dy), data(x), data(w), data(b), stats_.data_ptr<float>(), data(out[0]),
+                                  data(out[1]), data(out[2]), data(space), space.defined() ? space.numel() : 0, stream_of(x)));
+    return out;
   }
+
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    x_.reset_data();
+    w_.reset_data();
+    b_.reset_data();
+    stats_.reset();
+  }
+  std::string name() const override { return "LayerNormBackward"; }
+
+ private:
+  torch::autograd::SavedVariable x_, w_, b_;
+  Tensor stats_;
+  double eps_;
+  int64_t activation_;
+  at::ScalarType param_type_;
 };
 
-Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, int64_t activation) {
-  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
-  check_arguments(x, w, b);
-  const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) ||
-                                                   (b.defined() && b.requires_grad()));
-  if (!grad)
-    return forward(with_rows(x), w.defined() ? w.contiguous() : w, b.defined() ? b.contiguous() : b, eps, activation, nullptr);
+Tensor layer_norm(const Tensor& x_in, const OptTensor& weight, const OptTensor& bias, double eps, int64_t activation) {
+  const Tensor w_in = weight.value_or(Tensor()), b_in = bias.value_or(Tensor());
+  check_arguments(x_in, w_in, b_in);
+  // what is copied for its layout is copied where its gradient does not see it: the edges lead to the arguments themselves
+  std::optional<at::AutoDispatchBelowADInplaceOrView> plain(std::in_place);
+  const Tensor x = with_rows(x_in), w = w_in.defined() ? w_in.contiguous() : w_in, b = b_in.defined() ? b_in.contiguous() : b_in;
+  const bool grad = at::GradMode::is_enabled() && (x_in.requires_grad() || (w_in.defined() && w_in.requires_grad()) ||
+                                                   (b_in.defined() && b_in.requires_grad()));
+  if (!grad) return forward(x, w, b, eps, activation, nullptr);
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
-    for (const Tensor* t : {&x, &w, &b}) refuse_foreign_accumulator(*t);
-  return LayerNormFn::apply(x, w.defined() ? OptTensor(w) : OptTensor(), b.defined() ? OptTensor(b) : OptTensor(), eps, activation);
+    for (const Tensor* t : {&x_in, &w_in, &b_in}) refuse_foreign_accumulator(*t);
+  Tensor stats;
+  Tensor y = forward(x, w, b, eps, activation, &stats);
+  const auto param_type = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : at::kFloat;
+  auto node = std::shared_ptr<LayerNormBackward>(new LayerNormBackward(x, w, b, stats, eps, activation, param_type),
+                                                 torch::autograd::deleteNode);
+  plain.reset();
+  node->set_next_edges(torch::autograd::collect_next_edges(x_in, w_in, b_in));
+  torch::autograd::set_history(y, node);
+  return y;
 }
 
 // ------------------------------------------------------------------------------------------------ gradient norm
