@@ -63,7 +63,7 @@ struct NormArgs {
   int cols;
   int chunks;     // of a row that is longer than a workgroup's registers
   int param_f32;  // the parameters' type: f32, or the rows' type
-  float eps;
+  float eps, inv_cols;
 };
 
 template <class T>
@@ -83,7 +83,9 @@ struct Pack {
 // Which columns a thread of a row's group owns.  Vector v covers [v V, v V + V); the one that would reach past the row is moved
 // back to end with it and leaves out (`skip`) what the vector before it owns already, so every load is a whole one and none needs
 // a branch.  A vector that lies wholly past the row skips everything.
-template <int V, int TPR, bool EVEN>
+// The kernels for 8 threads and more are called for rows of more than half their capacity: the first half of a thread's vectors
+// needs no such care.
+template <int V, int TPR, int K, bool EVEN>
 struct Place {
   int col, skip;
   Place() = default;
@@ -92,7 +94,7 @@ struct Place {
     col = EVEN || at + V <= cols ? at : cols - V;
     skip = EVEN ? 0 : at - col;
   }
-  __device__ __forceinline__ bool owns(int i) const { return EVEN || i >= skip; }
+  __device__ __forceinline__ bool owns(int k, int i) const { return EVEN || (TPR >= 8 && 2 * k < K) || i >= skip; }
 };
 
 // Stores the elements that a thread owns.  A moved-back vector stores its own alone: what it has computed for its neighbour's
@@ -125,13 +127,16 @@ __device__ __forceinline__ void load_params(const NormArgs& a, const void* p, in
   }
 }
 
-// Sums of N numbers over the TPR threads that share a row, the same bits in each of them.  Groups of 16 and 64 stay in their
+// Sums of N numbers over the TPR threads that share a row, the same bits in each of them.  Groups of up to 64 stay in their
 // wavefront; larger ones (whole workgroups) exchange one number per wavefront through LDS.  Two buffers in turn make one barrier
 // per call enough: a wavefront can be at most one call ahead of another.
 template <int TPR, int N>
 __device__ __forceinline__ void sum_group(float (&v)[N], float* slots, int& turn) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = TPR == 16 ? sum16(v[i]) : sum64(v[i]);
+  for (int i = 0; i < N; ++i) {
+    if constexpr (TPR < 64) v[i] = sum_lanes<TPR>(v[i]);
+    else v[i] = sum64(v[i]);
+  }
   if constexpr (TPR > 64) {
     constexpr int W = TPR / 64;
     float* s = slots + turn * 2 * W;
@@ -151,43 +156,53 @@ __device__ __forceinline__ void sum_group(float (&v)[N], float* slots, int& turn
   }
 }
 
+// 1 / sqrt(variance + eps) to two units in the last place; the instruction takes no subnormal numbers, so small ones are scaled.
+__device__ __forceinline__ float inverse_deviation(float variance, float eps) {
+  const float v = (variance < 0 ? 0 : variance) + eps;  // NaN stays
+  const bool small = v < 0x1p-96f;
+  return __builtin_amdgcn_rsqf(small ? v * 0x1p64f : v) * (small ? 0x1p32f : 1.0f);
+}
+
 // Mean and 1 / sqrt(variance + eps) of the row whose elements the group's threads hold.  The variance is the mean square of
 // the deviations from the rounded mean; their sum, which would be zero but for that rounding, corrects both.
 template <int V, int TPR, int K, bool EVEN>
-__device__ __forceinline__ void statistics(const float (&x)[K][V], const Place<V, TPR, EVEN> (&at)[K], int cols, float eps,
+__device__ __forceinline__ void statistics(const float (&x)[K][V], const Place<V, TPR, K, EVEN> (&at)[K], float inv_n, float eps,
                                            float* slots, int& turn, float& mean, float& r) {
   float s[1] = {0};
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[0] += at[k].owns(i) ? x[k][i] : 0.0f;
+    for (int i = 0; i < V; ++i) s[0] += at[k].owns(k, i) ? x[k][i] : 0.0f;
   sum_group<TPR>(s, slots, turn);
-  const float n = (float)cols, first = s[0] / n;
+  const float first = s[0] * inv_n;
   float d[2] = {0, 0};
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float e = at[k].owns(i) ? x[k][i] - first : 0.0f;
+      const float e = at[k].owns(k, i) ? x[k][i] - first : 0.0f;
       d[0] += e;
       d[1] = __builtin_fmaf(e, e, d[1]);
     }
   sum_group<TPR>(d, slots, turn);
-  mean = first + d[0] / n;
-  float variance = (d[1] - d[0] * d[0] / n) / n;
-  variance = variance < 0 ? 0 : variance;  // NaN stays
-  r = 1.0f / __builtin_sqrtf(variance + eps);
+  const float off = d[0] * inv_n;
+  mean = first + off;
+  r = inverse_deviation(__builtin_fmaf(-off, d[0], d[1]) * inv_n, eps);
 }
+
+// Workgroup size: groups within a wavefront share workgroups of four, larger groups are workgroups.
+template <int TPR>
+constexpr int forward_threads() { return TPR <= 64 ? 256 : TPR; }
 
 // Forward, a row in the registers of TPR threads (K vectors of V elements each): read once, written once.
 template <class T, int V, int TPR, int K, bool EVEN, int ACT>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_forward_kernel(NormArgs a) {
-  constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
+__global__ __launch_bounds__(forward_threads<TPR>()) void layer_norm_forward_kernel(NormArgs a) {
+  constexpr int NT = forward_threads<TPR>(), RPB = NT / TPR;
   typedef typename Pack<T, V>::type vec;
   __shared__ float slots[TPR > 64 ? 4 * TPR / 64 : 1];
   int turn = 0;
   const int t = threadIdx.x % TPR;
-  Place<V, TPR, EVEN> at[K];
+  Place<V, TPR, K, EVEN> at[K];
   const int64_t step = (int64_t)gridDim.x * RPB;
   int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
   if (row >= a.rows) return;  // whole groups; of a group of more than a wavefront there is one to a workgroup
@@ -195,7 +210,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_forward_kern
   float w[K][V], b[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    at[k] = Place<V, TPR, EVEN>(t, k, a.cols);
+    at[k] = Place<V, TPR, K, EVEN>(t, k, a.cols);
     if (KEEP) {
       load_params<T, V>(a, a.w, at[k].col, 1.0f, w[k]);
       load_params<T, V>(a, a.b, at[k].col, 0.0f, b[k]);
@@ -214,7 +229,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_forward_kern
 #pragma unroll
     for (int k = 0; k < K; ++k) next[k] = *(const vec*)((const T*)a.x + ahead * a.x_stride + at[k].col);
     float mean, r;
-    statistics<V, TPR, K, EVEN>(x, at, a.cols, a.eps, slots, turn, mean, r);
+    statistics<V, TPR, K, EVEN>(x, at, a.inv_cols, a.eps, slots, turn, mean, r);
     T* y = (T*)a.y + row * a.cols;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -290,8 +305,7 @@ __device__ __forceinline__ void join_chunks(const NormArgs& a, int64_t row, floa
     const float d = p[c].x - mean;
     q += __builtin_fmaf(d * d, (float)min(a.cols - c * chunk_cols<V>(), chunk_cols<V>()), p[c].y);
   }
-  const float variance = sum64(q) / n;
-  r = 1.0f / __builtin_sqrtf((variance < 0 ? 0 : variance) + a.eps);
+  r = inverse_deviation(sum64(q) / n, a.eps);
 }
 
 template <class T, int V, int ACT>
@@ -357,14 +371,14 @@ __global__ __launch_bounds__(backward_threads<TPR>()) void layer_norm_backward_k
   __shared__ float joined[SUMS && TPR <= 64 ? 2 * TPR * K * V : 1];
   int turn = 0;
   const int t = threadIdx.x % TPR;
-  Place<V, TPR, EVEN> at[K];
+  Place<V, TPR, K, EVEN> at[K];
   const int64_t step = (int64_t)gridDim.x * RPB;
   int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
   constexpr bool KEEP = K * V <= 16;
   float w[K][V], b[K][V], dw[K][V], db[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    at[k] = Place<V, TPR, EVEN>(t, k, a.cols);
+    at[k] = Place<V, TPR, K, EVEN>(t, k, a.cols);
     if (KEEP) {
       load_params<T, V>(a, a.w, at[k].col, 1.0f, w[k]);
       if (ACT != RBL_ACT_NONE) load_params<T, V>(a, a.b, at[k].col, 0.0f, b[k]);
@@ -388,7 +402,7 @@ __global__ __launch_bounds__(backward_threads<TPR>()) void layer_norm_backward_k
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           h[k][i] = ((float)next_x[k][i] - mean) * r;
-          g[k][i] = at[k].owns(i) ? (float)next_dy[k][i] : 0.0f;
+          g[k][i] = at[k].owns(k, i) ? (float)next_dy[k][i] : 0.0f;
         }
       const int64_t ahead = row + step < a.rows ? row + step : row;
       next_s = *(const float2*)(a.stats + 2 * ahead);
@@ -418,7 +432,7 @@ __global__ __launch_bounds__(backward_threads<TPR>()) void layer_norm_backward_k
       }
       if (a.dx) {
         sum_group<TPR>(s, slots, turn);
-        const float p = s[0] / (float)a.cols, q = s[1] / (float)a.cols;
+        const float p = s[0] * a.inv_cols, q = s[1] * a.inv_cols;
         T* dx = (T*)a.dx + row * a.cols;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -440,19 +454,19 @@ __global__ __launch_bounds__(backward_threads<TPR>()) void layer_norm_backward_k
         put_sums<V, EVEN>(out + width + at[k].col, db[k], at[k].skip);
       }
     } else {
-      // the groups add their sums up one after the other
+      // the wavefronts add their sums up one after the other
       constexpr int GROUPS = NT / 64;
-      if (TPR == 16) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          dw[0][i] += __shfl_xor(dw[0][i], 16);
-          dw[0][i] += __shfl_xor(dw[0][i], 32);
-          db[0][i] += __shfl_xor(db[0][i], 16);
-          db[0][i] += __shfl_xor(db[0][i], 32);
-        }
-      }
+      for (int d = TPR; d < 64; d *= 2)
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            dw[k][i] += __shfl_xor(dw[k][i], d);
+            db[k][i] += __shfl_xor(db[k][i], d);
+          }
       for (int group = 0; group < GROUPS; ++group) {
-        if ((int)threadIdx.x / 64 == group && (TPR == 64 || threadIdx.x % 64 < 16)) {
+        if ((int)threadIdx.x / 64 == group && threadIdx.x % 64 < TPR) {
 #pragma unroll
           for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -472,7 +486,7 @@ __global__ __launch_bounds__(backward_threads<TPR>()) void layer_norm_backward_k
       }
       for (int j = threadIdx.x; j < 2 * TPR * K; j += NT) {
         const int which = j / (TPR * K), v = j % (TPR * K), k = v / TPR;
-        const Place<V, TPR, EVEN> place(v % TPR, k, a.cols);
+        const Place<V, TPR, K, EVEN> place(v % TPR, k, a.cols);
         float sum[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) sum[i] = joined[which * TPR * K * V + (k * V + i) * TPR + v % TPR];
@@ -625,15 +639,30 @@ __global__ __launch_bounds__(kThreads) void layer_norm_chunk_backward_kernel(Nor
 
 constexpr int kCus = 256;
 
-template <class T, int V, int TPR, int K, int ACT>
-void forward_rows(NormArgs a, hipStream_t st) {
-  constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
-  // as many workgroups as the chip holds at once, each with its share of the rows
-  const int64_t need = (a.rows + RPB - 1) / RPB, most = (int64_t)kCus * (2048 / NT);
-  const void* kernel = a.cols == TPR * K * V ? (const void*)layer_norm_forward_kernel<T, V, TPR, K, true, ACT>
-                                             : (const void*)layer_norm_forward_kernel<T, V, TPR, K, false, ACT>;
+// Workgroups for `need` shares of work: what the chip holds at once of this kernel, or fewer, so that all have the same
+// number of shares but for one.
+unsigned even_grid(int64_t need, int64_t resident) {
+  const int64_t rounds = (need + resident - 1) / resident;
+  return (unsigned)((need + rounds - 1) / rounds);
+}
+int resident_groups(const void* kernel, int threads) {
+  int n = 0;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != hipSuccess || n < 1)
+    throw std::runtime_error("HIP error: occupancy of a kernel");
+  return n * kCus;
+}
+
+template <class T, int V, int TPR, int K, bool EVEN, int ACT>
+void forward_launch(NormArgs a, hipStream_t st) {
+  constexpr int NT = forward_threads<TPR>(), RPB = NT / TPR;
+  const void* kernel = (const void*)layer_norm_forward_kernel<T, V, TPR, K, EVEN, ACT>;
+  static const int resident = resident_groups(kernel, NT);
   void* args[] = {&a};
-  launch(kernel, (unsigned)(need < most ? need : most), NT, args, st);
+  launch(kernel, even_grid((a.rows + RPB - 1) / RPB, resident), NT, args, st);
+}
+template <class T, int V, int TPR, int K, int ACT>
+void forward_rows(const NormArgs& a, hipStream_t st) {
+  a.cols == TPR * K * V ? forward_launch<T, V, TPR, K, true, ACT>(a, st) : forward_launch<T, V, TPR, K, false, ACT>(a, st);
 }
 
 // The widest rows that a workgroup's registers hold, forward
@@ -649,24 +678,18 @@ template <class T, int ACT>
 void run_forward(NormArgs a, hipStream_t st) {
   constexpr int V = 16 / sizeof(T);
   if (a.rows == 0) return;
-  const int vectors = (a.cols + V - 1) / V;
-  if (a.cols < V) return forward_rows<T, 1, 16, 1, ACT>(a, st);
-  if (vectors <= 16) return forward_rows<T, V, 16, 1, ACT>(a, st);
-  if (vectors <= 64) return forward_rows<T, V, 64, 1, ACT>(a, st);
-  if (vectors <= 128) return forward_rows<T, V, 64, 2, ACT>(a, st);
-  // up to 16 elements to a thread: more do not fit into the registers without spilling
-  if constexpr (V == 4) {
-    if (vectors <= 256) return forward_rows<T, V, 64, 4, ACT>(a, st);
-    if (vectors <= 512) return forward_rows<T, V, 256, 2, ACT>(a, st);
-    if (vectors <= 1024) return forward_rows<T, V, 256, 4, ACT>(a, st);
-    if (vectors <= 2048) return forward_rows<T, V, 1024, 2, ACT>(a, st);
-    if (vectors <= 4096) return forward_rows<T, V, 1024, 4, ACT>(a, st);
-  } else {
-    if (vectors <= 256) return forward_rows<T, V, 256, 1, ACT>(a, st);
-    if (vectors <= 512) return forward_rows<T, V, 256, 2, ACT>(a, st);
-    if (vectors <= 1024) return forward_rows<T, V, 1024, 1, ACT>(a, st);
-    if (vectors <= 2048) return forward_rows<T, V, 1024, 2, ACT>(a, st);
-  }
+  // 16 elements to a thread: fewer leave too much of the work on a row's two sums, more spill out of the registers
+  constexpr int K = 16 / V;
+  if (a.cols < V) return forward_rows<T, 1, 4, 2, ACT>(a, st);
+  if (a.cols <= 64) return forward_rows<T, V, 4, K, ACT>(a, st);
+  if (a.cols <= 128) return forward_rows<T, V, 8, K, ACT>(a, st);
+  if (a.cols <= 256) return forward_rows<T, V, 16, K, ACT>(a, st);
+  if (a.cols <= 512) return forward_rows<T, V, 32, K, ACT>(a, st);
+  if (a.cols <= 1024) return forward_rows<T, V, 64, K, ACT>(a, st);
+  if (a.cols <= 2048) return forward_rows<T, V, 128, K, ACT>(a, st);
+  if (a.cols <= 4096) return forward_rows<T, V, 256, K, ACT>(a, st);
+  if (a.cols <= 8192) return forward_rows<T, V, 512, K, ACT>(a, st);
+  if (a.cols <= kForwardCols) return forward_rows<T, V, 1024, K, ACT>(a, st);
   a.chunks = chunk_count<T>(a.cols);
   const int64_t items = a.rows * a.chunks;
   const unsigned grid = (unsigned)(items < 1 << 20 ? items : 1 << 20);
@@ -676,29 +699,23 @@ void run_forward(NormArgs a, hipStream_t st) {
 }
 // Workgroups of the backward kernels, i.e. rows of partial sums
 struct BackwardPlan {
-  int vectors, tpr, k;  // tpr 0: chunks
-  int chunks;
+  int tpr;     // threads to a row; 0: rows in chunks
+  int chunks;  // of a row
   int64_t groups;
 };
+constexpr int kBackwardCols = 8192;
 
 BackwardPlan backward_plan(const rbl_layer_norm_shape& s) {
-  const int v = s.dtype == RBL_F32 ? 4 : 8;
   BackwardPlan p{};
-  p.vectors = (int)((s.cols + v - 1) / v);
-  if (s.cols < v || p.vectors <= 16) p.tpr = 16, p.k = 1;
-  else if (p.vectors <= 64) p.tpr = 64, p.k = 1;
-  else if (p.vectors <= 128) p.tpr = 64, p.k = 2;
-  else if (v == 4 && p.vectors <= 256) p.tpr = 64, p.k = 4;
-  else if (p.vectors <= 256) p.tpr = 256, p.k = 1;
-  else if (p.vectors <= 512) p.tpr = 256, p.k = 2;
-  else if (p.vectors <= 1024) p.tpr = 512, p.k = 2;
-  else if (v == 4 && p.vectors <= 2048) p.tpr = 512, p.k = 4;
-  if (p.tpr) {
+  if (s.cols <= kBackwardCols) {
+    p.tpr = 4;
+    while (p.tpr * 16 < s.cols) p.tpr *= 2;
     const int nt = p.tpr <= 64 ? 512 : p.tpr;
-    const int64_t need = (s.rows * p.tpr + nt - 1) / nt, most = (int64_t)kCus * (1024 / nt);
-    p.groups = need < most ? need : most;
+    const int64_t need = (s.rows * p.tpr + nt - 1) / nt;
+    p.groups = need == 0 ? 0 : even_grid(need, kCus * (int64_t)(1024 / nt));
   } else {
-    p.chunks = (int)((s.cols + kThreads * kChunkK * v - 1) / (kThreads * kChunkK * v));
+    const int chunk = kThreads * kChunkK * (s.dtype == RBL_F32 ? 4 : 8);
+    p.chunks = (int)((s.cols + chunk - 1) / chunk);
     const int64_t most = (kCus + p.chunks - 1) / p.chunks;
     p.groups = s.rows < most ? s.rows : most;
   }
@@ -718,18 +735,18 @@ void backward_rows(NormArgs a, const BackwardPlan& p, bool sums, hipStream_t st)
 
 template <class T, int ACT>
 void run_backward(NormArgs a, const BackwardPlan& p, hipStream_t st) {
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T), K = 16 / V;
   const bool sums = a.dw || a.db;
   if (a.rows > 0 && (a.dx || sums)) {
-    if (a.cols < V) backward_rows<T, 1, 16, 1, ACT>(a, p, sums, st);
-    else if (p.tpr == 16) backward_rows<T, V, 16, 1, ACT>(a, p, sums, st);
-    else if (p.tpr == 64 && p.k == 1) backward_rows<T, V, 64, 1, ACT>(a, p, sums, st);
-    else if (p.tpr == 64 && p.k == 2) backward_rows<T, V, 64, 2, ACT>(a, p, sums, st);
-    else if (p.tpr == 64) { if constexpr (V == 4) backward_rows<T, V, 64, 4, ACT>(a, p, sums, st); }
-    else if (p.tpr == 256 && p.k == 1) { if constexpr (V == 8) backward_rows<T, V, 256, 1, ACT>(a, p, sums, st); }
-    else if (p.tpr == 256) backward_rows<T, V, 256, 2, ACT>(a, p, sums, st);
-    else if (p.tpr == 512 && p.k == 2) backward_rows<T, V, 512, 2, ACT>(a, p, sums, st);
-    else if (p.tpr == 512) { if constexpr (V == 4) backward_rows<T, V, 512, 4, ACT>(a, p, sums, st); }
+    if (a.cols < V) backward_rows<T, 1, 4, 2, ACT>(a, p, sums, st);
+    else if (p.tpr == 4) backward_rows<T, V, 4, K, ACT>(a, p, sums, st);
+    else if (p.tpr == 8) backward_rows<T, V, 8, K, ACT>(a, p, sums, st);
+    else if (p.tpr == 16) backward_rows<T, V, 16, K, ACT>(a, p, sums, st);
+    else if (p.tpr == 32) backward_rows<T, V, 32, K, ACT>(a, p, sums, st);
+    else if (p.tpr == 64) backward_rows<T, V, 64, K, ACT>(a, p, sums, st);
+    else if (p.tpr == 128) backward_rows<T, V, 128, K, ACT>(a, p, sums, st);
+    else if (p.tpr == 256) backward_rows<T, V, 256, K, ACT>(a, p, sums, st);
+    else if (p.tpr == 512) backward_rows<T, V, 512, K, ACT>(a, p, sums, st);
     else {
       a.chunks = p.chunks;
       const int64_t items = a.rows * a.chunks;
@@ -792,6 +809,7 @@ NormArgs args_of(const rbl_layer_norm_shape& s) {
   a.x_stride = s.x_stride;
   a.dy_stride = s.dy_stride;
   a.cols = (int)s.cols;
+  a.inv_cols = 1.0f / (float)s.cols;
   a.param_f32 = s.param_dtype == RBL_F32;
   a.eps = s.eps;
   return a;

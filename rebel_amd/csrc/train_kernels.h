@@ -66,18 +66,27 @@ __device__ __forceinline__ float dpp(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
 }
 
-// Sum over the 16 lanes of a DPP row; every lane gets the same bits (each step adds the same two numbers on both sides).
-__device__ __forceinline__ float sum16(float v) {
-  v += dpp<0xB1>(v);   // quad_perm [1,0,3,2]
-  v += dpp<0x4E>(v);   // quad_perm [2,3,0,1]
-  v += dpp<0x141>(v);  // row_half_mirror
-  v += dpp<0x140>(v);  // row_mirror
+// Sum over the 2^k neighbouring lanes that share a row (4, 8, 16 or 32); every lane gets the same bits, since each step adds the
+// same two numbers on both sides.
+template <int LANES>
+__device__ __forceinline__ float sum_lanes(float v) {
+  static_assert(LANES == 4 || LANES == 8 || LANES == 16 || LANES == 32);
+  v += dpp<0xB1>(v);                     // quad_perm [1,0,3,2]
+  v += dpp<0x4E>(v);                     // quad_perm [2,3,0,1]
+  if (LANES >= 8) v += dpp<0x141>(v);    // row_half_mirror
+  if (LANES >= 16) v += dpp<0x140>(v);   // row_mirror
+  if (LANES >= 32) {
+    // v_permlane16_swap exchanges the odd rows of 16 lanes of one register with the even ones of another: copy, swap, add
+    float c;
+    asm("v_mov_b32 %1, %0\n\ts_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(v), "=&v"(c));
+    v += c;
+  }
   return v;
 }
 
 // Sum over the wavefront, the same bits in every lane: four DPP rows, whose sums go through scalar registers.
 __device__ __forceinline__ float sum64(float v) {
-  v = sum16(v);
+  v = sum_lanes<16>(v);
   const int i = __builtin_bit_cast(int, v);
   const float a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 0)),
               b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 16)),
