@@ -94,7 +94,7 @@ struct Place {
     col = EVEN || at + V <= cols ? at : cols - V;
     skip = EVEN ? 0 : at - col;
   }
-  __device__ __forceinline__ bool owns(int k, int i) const { return EVEN || (TPR >= 8 && 2 * k < K) || i >= skip; }
+  __device__ __forceinline__ bool owns(int k, int i) const { return EVEN || (TPR >= 8 && 2 * k + 2 <= K) || i >= skip; }
 };
 
 // Stores the elements that a thread owns.  A moved-back vector stores its own alone: what it has computed for its neighbour's
@@ -341,10 +341,11 @@ __global__ __launch_bounds__(kThreads) void layer_norm_chunk_forward_kernel(Norm
   }
 }
 
-// Workgroup size of the backward kernel: rows of up to 64 threads share a workgroup of eight wavefronts, so that fewer
-// partial sums of the parameters' gradients leave it.
-template <int TPR>
-constexpr int backward_threads() { return TPR <= 64 ? 512 : TPR; }
+// Workgroup size of the backward kernel, as forward.  Eight wavefronts to a CU are the best number at every width (more slow the
+// three streams down and leave more partial sums: 270336 x 256 f32 + GELU 150 us with 8, 167 with 16, 178 with 32; 8192 x 4096 bf16
+// 44 / 48 / 56 us).
+constexpr int backward_threads(int tpr) { return tpr <= 64 ? 256 : tpr; }
+constexpr int kBackwardWaves = 8;
 
 // Writes what a thread has summed up over rows for its V columns: the owned ones alone.
 template <int V, bool EVEN>
@@ -364,8 +365,8 @@ __device__ __forceinline__ void put_sums(float* out, const float (&v)[V], int sk
 // Backward, a row in the registers of TPR threads: x and dy are read once, dx is written, and (SUMS) g h and g are summed up over
 // the rows of the workgroup, in registers; the workgroups' sums are joined by layer_norm_sums_kernel.
 template <class T, int V, int TPR, int K, bool EVEN, int ACT, bool SUMS>
-__global__ __launch_bounds__(backward_threads<TPR>()) void layer_norm_backward_kernel(NormArgs a) {
-  constexpr int NT = backward_threads<TPR>(), RPB = NT / TPR;
+__global__ __launch_bounds__(backward_threads(TPR)) void layer_norm_backward_kernel(NormArgs a) {
+  constexpr int NT = backward_threads(TPR), RPB = NT / TPR;
   typedef typename Pack<T, V>::type vec;
   __shared__ float slots[TPR > 64 ? 4 * TPR / 64 : 1];
   __shared__ float joined[SUMS && TPR <= 64 ? 2 * TPR * K * V : 1];
@@ -496,34 +497,38 @@ __global__ __launch_bounds__(backward_threads<TPR>()) void layer_norm_backward_k
   }
 }
 
-// The parameters' gradients from `count` rows of partial sums, each [2][width]: 64 columns to a workgroup, 64 threads down the
-// rows, in an order that depends on the counts alone.
+// The parameters' gradients from `count` rows of partial sums, each [2][width]: COLS columns to a workgroup, the other threads
+// down the rows, in an order that depends on the counts alone.  16 columns where there are few (64-byte accesses, but four times
+// the workgroups), else 64.
 constexpr int kSumsThreads = 1024;
-template <class T>
+template <class T, int COLS>
 __global__ __launch_bounds__(kSumsThreads) void layer_norm_sums_kernel(NormArgs a, int count) {
-  __shared__ float part[kSumsThreads / 64][64];
+  constexpr int LANES = COLS / 4, SLICES = kSumsThreads / LANES;
+  __shared__ float part[kSumsThreads / 64][COLS];
   const int width = (a.cols + 3) / 4 * 4;
-  const int quad = threadIdx.x % 16, slice = threadIdx.x / 16;
-  const int64_t col = (int64_t)blockIdx.x * 64 + quad * 4;
+  const int quad = threadIdx.x % LANES, slice = threadIdx.x / LANES;
+  const int64_t col = (int64_t)blockIdx.x * COLS + quad * 4;
   typedef Pack<float, 4>::type vec;
   float s[4] = {0, 0, 0, 0};
   if (col < 2 * (int64_t)width) {
 #pragma unroll 4
-    for (int g = slice; g < count; g += kSumsThreads / 16) {
+    for (int g = slice; g < count; g += SLICES) {
       const vec v = *(const vec*)(a.partial + (int64_t)g * 2 * width + col);
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[i] += v[i];
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    s[i] += __shfl_xor(s[i], 16);
-    s[i] += __shfl_xor(s[i], 32);
-    if (threadIdx.x % 64 < 16) part[threadIdx.x / 64][quad * 4 + i] = s[i];
+  for (int d = LANES; d < 64; d *= 2)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] += __shfl_xor(s[i], d);
+  if (threadIdx.x % 64 < LANES) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[threadIdx.x / 64][quad * 4 + i] = s[i];
   }
   lds_barrier();
-  const int64_t mine = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  if (threadIdx.x < 64 && mine < 2 * (int64_t)width) {
+  const int64_t mine = (int64_t)blockIdx.x * COLS + threadIdx.x;
+  if (threadIdx.x < COLS && mine < 2 * (int64_t)width) {
     float v = part[0][threadIdx.x];
 #pragma unroll
     for (int k = 1; k < kSumsThreads / 64; ++k) v += part[k][threadIdx.x];
@@ -708,11 +713,11 @@ constexpr int kBackwardCols = 8192;
 BackwardPlan backward_plan(const rbl_layer_norm_shape& s) {
   BackwardPlan p{};
   if (s.cols <= kBackwardCols) {
-    p.tpr = 4;
-    while (p.tpr * 16 < s.cols) p.tpr *= 2;
-    const int nt = p.tpr <= 64 ? 512 : p.tpr;
+    p.tpr = s.cols <= 32 ? 4 : 8;
+    while (p.tpr < 512 && p.tpr * 8 < s.cols) p.tpr *= 2;
+    const int nt = backward_threads(p.tpr);
     const int64_t need = (s.rows * p.tpr + nt - 1) / nt;
-    p.groups = need == 0 ? 0 : even_grid(need, kCus * (int64_t)(1024 / nt));
+    p.groups = need == 0 ? 0 : even_grid(need, (int64_t)kCus * kBackwardWaves * 64 / nt);
   } else {
     const int chunk = kThreads * kChunkK * (s.dtype == RBL_F32 ? 4 : 8);
     p.chunks = (int)((s.cols + chunk - 1) / chunk);
@@ -730,12 +735,13 @@ void backward_rows(NormArgs a, const BackwardPlan& p, bool sums, hipStream_t st)
                        : even ? (const void*)layer_norm_backward_kernel<T, V, TPR, K, true, ACT, false>
                               : (const void*)layer_norm_backward_kernel<T, V, TPR, K, false, ACT, false>;
   void* args[] = {&a};
-  launch(kernel, (unsigned)p.groups, backward_threads<TPR>(), args, st);
+  launch(kernel, (unsigned)p.groups, backward_threads(TPR), args, st);
 }
 
 template <class T, int ACT>
 void run_backward(NormArgs a, const BackwardPlan& p, hipStream_t st) {
-  constexpr int V = 16 / sizeof(T), K = 16 / V;
+  // 8 elements to a thread, 16 in the widest rows: x, dy, the parameters and both sums have to fit into its registers
+  constexpr int V = 16 / sizeof(T), K = 8 / V;
   const bool sums = a.dw || a.db;
   if (a.rows > 0 && (a.dx || sums)) {
     if (a.cols < V) backward_rows<T, 1, 4, 2, ACT>(a, p, sums, st);
@@ -746,7 +752,8 @@ void run_backward(NormArgs a, const BackwardPlan& p, hipStream_t st) {
     else if (p.tpr == 64) backward_rows<T, V, 64, K, ACT>(a, p, sums, st);
     else if (p.tpr == 128) backward_rows<T, V, 128, K, ACT>(a, p, sums, st);
     else if (p.tpr == 256) backward_rows<T, V, 256, K, ACT>(a, p, sums, st);
-    else if (p.tpr == 512) backward_rows<T, V, 512, K, ACT>(a, p, sums, st);
+    else if (p.tpr == 512 && a.cols <= 4096) backward_rows<T, V, 512, K, ACT>(a, p, sums, st);
+    else if (p.tpr == 512) backward_rows<T, V, 512, 2 * K, ACT>(a, p, sums, st);
     else {
       a.chunks = p.chunks;
       const int64_t items = a.rows * a.chunks;
@@ -765,7 +772,9 @@ void run_backward(NormArgs a, const BackwardPlan& p, hipStream_t st) {
     int count = (int)p.groups;
     void* args[] = {&a, &count};
     const int64_t width = (a.cols + 3) / 4 * 4;
-    launch((const void*)layer_norm_sums_kernel<T>, (unsigned)((2 * width + 63) / 64), kSumsThreads, args, st);
+    const bool few = 2 * width < 64 * kCus / 2;
+    launch(few ? (const void*)layer_norm_sums_kernel<T, 16> : (const void*)layer_norm_sums_kernel<T, 64>,
+           (unsigned)((2 * width + (few ? 15 : 63)) / (few ? 16 : 64)), kSumsThreads, args, st);
   }
 }
 
