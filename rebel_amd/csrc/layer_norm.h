@@ -1,0 +1,75 @@
+// rebel_amd/csrc/layer_norm.h -- layer normalisation, host side: what the entries (layer_norm.hip) and the kernels' launchers
+// (layer_norm_kernel.h, compiled once for each element type) share.
+#pragma once
+#include "train_kernels.h"
+
+namespace rbl {
+
+constexpr int kCus = 256;
+
+struct NormArgs {
+  const void *x, *dy, *w, *b;
+  void *y, *dx, *dw, *db;
+  float* stats;    // [rows][2]: mean, 1 / sqrt(variance + eps)
+  int64_t rows, x_stride, dy_stride;
+  float* partial;   // workspace: statistics of chunks (forward), sums of the parameters' gradients (backward)
+  float* row_sums;  // workspace: chunks' sums of g w and g w h
+  int cols;
+  int chunks;     // of a row that is longer than a workgroup's registers
+  int param_f32;  // the parameters' type: f32, or the rows' type
+  float eps, inv_cols;
+};
+
+// The widest rows that a workgroup's registers hold, forward
+constexpr int kForwardCols = 16384;
+
+// Longer ones go in chunks of kChunkK vectors to each of kThreads threads.
+constexpr int kThreads = 256, kChunkK = 4;
+inline int chunks_of_row(int64_t cols, int elements_of_vector) {
+  const int64_t chunk = kThreads * kChunkK * elements_of_vector;
+  return (int)((cols + chunk - 1) / chunk);
+}
+
+// Workgroups for `need` shares of work: what the chip holds at once of this kernel, or fewer, so that all have the same
+// number of shares but for one.
+inline unsigned even_grid(int64_t need, int64_t resident) {
+  const int64_t rounds = (need + resident - 1) / resident;
+  return (unsigned)((need + rounds - 1) / rounds);
+}
+// Workgroup size of the backward kernel, as forward.  Eight wavefronts to a CU are the best number at every width (more slow the
+// three streams down and leave more partial sums: 270336 x 256 f32 + GELU 150 us with 8, 167 with 16, 178 with 32; 8192 x 4096 bf16
+// 44 / 48 / 56 us).
+constexpr int backward_threads(int tpr) { return tpr <= 64 ? 256 : tpr; }
+constexpr int kBackwardWaves = 8;
+
+// Workgroups of the backward kernels, i.e. rows of partial sums
+struct BackwardPlan {
+  int tpr;     // threads to a row; 0: rows in chunks
+  int chunks;  // of a row
+  int64_t groups;
+};
+constexpr int kBackwardCols = 8192;
+
+inline BackwardPlan backward_plan(const rbl_layer_norm_shape& s) {
+  BackwardPlan p{};
+  if (s.cols <= kBackwardCols) {
+    p.tpr = s.cols <= 32 ? 4 : 8;
+    while (p.tpr < 512 && p.tpr * 8 < s.cols) p.tpr *= 2;
+    const int nt = backward_threads(p.tpr);
+    const int64_t need = (s.rows * p.tpr + nt - 1) / nt;
+    p.groups = need == 0 ? 0 : even_grid(need, (int64_t)kCus * kBackwardWaves * 64 / nt);
+  } else {
+    p.chunks = chunks_of_row(s.cols, s.dtype == RBL_F32 ? 4 : 8);
+    const int64_t most = (kCus + p.chunks - 1) / p.chunks;
+    p.groups = s.rows < most ? s.rows : most;
+  }
+  return p;
+}
+
+// Enqueue the passes; T: float, _Float16 or __bf16.
+template <class T>
+void layer_norm_forward(const NormArgs& a, int activation, hipStream_t st);
+template <class T>
+void layer_norm_backward(const NormArgs& a, const BackwardPlan& p, int activation, hipStream_t st);
+
+}  // namespace rbl

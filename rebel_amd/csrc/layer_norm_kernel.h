@@ -1,4 +1,4 @@
-// rebel_amd/csrc/layer_norm_kernel.hip -- layer normalisation, forward and backward, with an optional GELU behind it.
+// rebel_amd/csrc/layer_norm_kernel.h -- kernels of layer normalisation, forward and backward, with an optional GELU behind it.
 //
 // Row x of n values, weight w, bias b, eps e:
 //     m = sum x / n     v = sum (x - m)^2 / n     r = 1 / sqrt(v + e)     h = (x - m) r     z = h w + b
@@ -7,12 +7,14 @@
 //     db = sum_rows g     dw = sum_rows g h     dx = r (g w - sum(g w) / n - h sum(g w h) / n)
 //
 // h is computed again from x and the two statistics of the row, so nothing else is kept between the passes.
-#include "train_kernels.h"
+//
+// The element types are compiled apart (layer_norm_f32.hip, layer_norm_f16.hip, layer_norm_bf16.hip); layer_norm.hip holds the C
+// entries.
+#pragma once
+#include "layer_norm.h"
 
 namespace rbl {
 namespace {
-
-constexpr int kThreads = 256;
 
 // Phi(z) and exp(-z^2 / 2).  For x = |z|: Phi(-x) = exp(-x^2 / 2) P(x) with P(x) = exp(x^2 / 2) erfc(x / sqrt 2) / 2, which
 // falls smoothly from 1/2 like 1 / (x sqrt(2 pi)): a polynomial of degree 8 in u = 1 / (1 + 0.3 x) without a constant term
@@ -53,19 +55,6 @@ __device__ __forceinline__ float activate_slope(float z) {
   return __builtin_fmaf(z * 0.39894228f, e, phi);  // 1 / sqrt(2 pi)
 }
 
-struct NormArgs {
-  const void *x, *dy, *w, *b;
-  void *y, *dx, *dw, *db;
-  float* stats;    // [rows][2]: mean, 1 / sqrt(variance + eps)
-  int64_t rows, x_stride, dy_stride;
-  float* partial;   // workspace: statistics of chunks (forward), sums of the parameters' gradients (backward)
-  float* row_sums;  // workspace: chunks' sums of g w and g w h
-  int cols;
-  int chunks;     // of a row that is longer than a workgroup's registers
-  int param_f32;  // the parameters' type: f32, or the rows' type
-  float eps, inv_cols;
-};
-
 template <class T>
 __device__ __forceinline__ void put_param(const NormArgs& a, void* p, int col, float v) {
   if (a.param_f32)
@@ -99,16 +88,29 @@ struct Place {
 
 // Stores the elements that a thread owns.  A moved-back vector stores its own alone: what it has computed for its neighbour's
 // may differ in the last bit, since the compiler need not round the same way at another place of the vector.
-template <bool EVEN, class T, class VEC>
-__device__ __forceinline__ void put_row(T* out, const VEC& v, int skip) {
-  constexpr int V = sizeof(VEC) / sizeof(T);
+template <class T, int V, bool EVEN, bool STREAM>
+__device__ __forceinline__ void put_row(T* out, typename Pack<T, V>::type v, int skip) {
+  typedef typename Pack<T, V>::type vec;
   if (EVEN || skip == 0) {
-    *(VEC*)out = v;
+    if (STREAM)
+      __builtin_nontemporal_store(v, (vec*)out);
+    else
+      *(vec*)out = v;
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (i >= skip) out[i] = v[i];
   }
+}
+
+// A row's vectors.  STREAM: without a claim to the caches, for tensors that they cannot hold anyway.
+template <class T, int V, bool STREAM, class PLACE, int K>
+__device__ __forceinline__ void load_row(typename Pack<T, V>::type (&v)[K], const void* base, int64_t offset, const PLACE (&at)[K]) {
+  typedef typename Pack<T, V>::type vec;
+  const T* row = (const T*)base + offset;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    v[k] = STREAM ? __builtin_nontemporal_load((const vec*)(row + at[k].col)) : *(const vec*)(row + at[k].col);
 }
 
 template <class T, int V>
@@ -195,7 +197,7 @@ template <int TPR>
 constexpr int forward_threads() { return TPR <= 64 ? 256 : TPR; }
 
 // Forward, a row in the registers of TPR threads (K vectors of V elements each): read once, written once.
-template <class T, int V, int TPR, int K, bool EVEN, int ACT>
+template <class T, int V, int TPR, int K, bool EVEN, int ACT, bool STREAM>
 __global__ __launch_bounds__(forward_threads<TPR>()) void layer_norm_forward_kernel(NormArgs a) {
   constexpr int NT = forward_threads<TPR>(), RPB = NT / TPR;
   typedef typename Pack<T, V>::type vec;
@@ -217,8 +219,7 @@ __global__ __launch_bounds__(forward_threads<TPR>()) void layer_norm_forward_ker
     }
   }
   vec next[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) next[k] = *(const vec*)((const T*)a.x + row * a.x_stride + at[k].col);
+  load_row<T, V, STREAM>(next, a.x, row * a.x_stride, at);
   for (; row < a.rows; row += step) {
     float x[K][V];
 #pragma unroll
@@ -226,8 +227,7 @@ __global__ __launch_bounds__(forward_threads<TPR>()) void layer_norm_forward_ker
 #pragma unroll
       for (int i = 0; i < V; ++i) x[k][i] = (float)next[k][i];
     const int64_t ahead = row + step < a.rows ? row + step : row;  // the next row is on its way while this one is computed
-#pragma unroll
-    for (int k = 0; k < K; ++k) next[k] = *(const vec*)((const T*)a.x + ahead * a.x_stride + at[k].col);
+    load_row<T, V, STREAM>(next, a.x, ahead * a.x_stride, at);
     float mean, r;
     statistics<V, TPR, K, EVEN>(x, at, a.inv_cols, a.eps, slots, turn, mean, r);
     T* y = (T*)a.y + row * a.cols;
@@ -240,7 +240,7 @@ __global__ __launch_bounds__(forward_threads<TPR>()) void layer_norm_forward_ker
       vec out;
 #pragma unroll
       for (int i = 0; i < V; ++i) out[i] = (T)activate<ACT>(__builtin_fmaf((x[k][i] - mean) * r, w[k][i], b[k][i]));
-      put_row<EVEN>(y + at[k].col, out, at[k].skip);
+      put_row<T, V, EVEN, STREAM>(y + at[k].col, out, at[k].skip);
     }
     if (a.stats && t == 0) *(float2*)(a.stats + 2 * row) = make_float2(mean, r);
   }
@@ -248,7 +248,6 @@ __global__ __launch_bounds__(forward_threads<TPR>()) void layer_norm_forward_ker
 
 // Rows that are longer than a workgroup's registers: chunks of kChunk vectors, each with its own mean and sum of squared
 // deviations, which the second kernel joins (Chan's formula) before it normalises its chunk.
-constexpr int kChunkK = 4;
 template <int V>
 constexpr int chunk_cols() { return kThreads * kChunkK * V; }
 
@@ -335,17 +334,11 @@ __global__ __launch_bounds__(kThreads) void layer_norm_chunk_forward_kernel(Norm
       vec out;
 #pragma unroll
       for (int i = 0; i < V; ++i) out[i] = (T)activate<ACT>(__builtin_fmaf(((float)p[k][i] - mean) * r, w[i], b[i]));
-      put_row<false>(y + col[k], out, (threadIdx.x + k * kThreads) * V - col[k]);
+      put_row<T, V, false, false>(y + col[k], out, (threadIdx.x + k * kThreads) * V - col[k]);
     }
     if (a.stats && begin == 0 && threadIdx.x == 0) *(float2*)(a.stats + 2 * row) = make_float2(mean, r);
   }
 }
-
-// Workgroup size of the backward kernel, as forward.  Eight wavefronts to a CU are the best number at every width (more slow the
-// three streams down and leave more partial sums: 270336 x 256 f32 + GELU 150 us with 8, 167 with 16, 178 with 32; 8192 x 4096 bf16
-// 44 / 48 / 56 us).
-constexpr int backward_threads(int tpr) { return tpr <= 64 ? 256 : tpr; }
-constexpr int kBackwardWaves = 8;
 
 // Writes what a thread has summed up over rows for its V columns: the owned ones alone.
 template <int V, bool EVEN>
@@ -364,7 +357,7 @@ __device__ __forceinline__ void put_sums(float* out, const float (&v)[V], int sk
 
 // Backward, a row in the registers of TPR threads: x and dy are read once, dx is written, and (SUMS) g h and g are summed up over
 // the rows of the workgroup, in registers; the workgroups' sums are joined by layer_norm_sums_kernel.
-template <class T, int V, int TPR, int K, bool EVEN, int ACT, bool SUMS>
+template <class T, int V, int TPR, int K, bool EVEN, int ACT, bool SUMS, bool STREAM>
 __global__ __launch_bounds__(backward_threads(TPR)) void layer_norm_backward_kernel(NormArgs a) {
   constexpr int NT = backward_threads(TPR), RPB = NT / TPR;
   typedef typename Pack<T, V>::type vec;
@@ -390,11 +383,8 @@ __global__ __launch_bounds__(backward_threads(TPR)) void layer_norm_backward_ker
   if (row < a.rows) {
     vec next_x[K], next_dy[K];
     float2 next_s = *(const float2*)(a.stats + 2 * row);
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      next_x[k] = *(const vec*)((const T*)a.x + row * a.x_stride + at[k].col);
-      next_dy[k] = *(const vec*)((const T*)a.dy + row * a.dy_stride + at[k].col);
-    }
+    load_row<T, V, STREAM>(next_x, a.x, row * a.x_stride, at);
+    load_row<T, V, STREAM>(next_dy, a.dy, row * a.dy_stride, at);
     for (; row < a.rows; row += step) {
       const float mean = next_s.x, r = next_s.y;
       float h[K][V], g[K][V];
@@ -407,11 +397,8 @@ __global__ __launch_bounds__(backward_threads(TPR)) void layer_norm_backward_ker
         }
       const int64_t ahead = row + step < a.rows ? row + step : row;
       next_s = *(const float2*)(a.stats + 2 * ahead);
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        next_x[k] = *(const vec*)((const T*)a.x + ahead * a.x_stride + at[k].col);
-        next_dy[k] = *(const vec*)((const T*)a.dy + ahead * a.dy_stride + at[k].col);
-      }
+      load_row<T, V, STREAM>(next_x, a.x, ahead * a.x_stride, at);
+      load_row<T, V, STREAM>(next_dy, a.dy, ahead * a.dy_stride, at);
       float s[2] = {0, 0};
 #pragma unroll
       for (int k = 0; k < K; ++k) {
@@ -440,7 +427,7 @@ __global__ __launch_bounds__(backward_threads(TPR)) void layer_norm_backward_ker
           vec out;
 #pragma unroll
           for (int i = 0; i < V; ++i) out[i] = (T)(r * (g[k][i] - __builtin_fmaf(h[k][i], q, p)));
-          put_row<EVEN>(dx + at[k].col, out, at[k].skip);
+          put_row<T, V, EVEN, STREAM>(dx + at[k].col, out, at[k].skip);
         }
       }
     }
@@ -628,7 +615,7 @@ __global__ __launch_bounds__(kThreads) void layer_norm_chunk_backward_kernel(Nor
         }
         out[i] = (T)(st.y * (g * w[i] - __builtin_fmaf(h, q, p)));
       }
-      if (a.dx) put_row<false>(dx + col[k], out, skip[k]);
+      if (a.dx) put_row<T, V, false, false>(dx + col[k], out, skip[k]);
     }
   }
   if constexpr (SUMS) {
@@ -642,14 +629,14 @@ __global__ __launch_bounds__(kThreads) void layer_norm_chunk_backward_kernel(Nor
   }
 }
 
-constexpr int kCus = 256;
+// A tensor of this size leaves nothing in the cache of 256 MB that its next reader could use: past the caches, 32768 x 8192 bf16
+// takes 181 instead of 197 us forward, 276 instead of 292 us backward.  With smaller ones the reader would pay (16384 x 2048 bf16
+// and a pass over its result: 48 instead of 43 us).
+constexpr int64_t kStreamBytes = (int64_t)512 << 20;
+template <class T>
+bool beyond_caches(const NormArgs& a) { return a.rows * a.cols * (int64_t)sizeof(T) >= kStreamBytes; }
 
-// Workgroups for `need` shares of work: what the chip holds at once of this kernel, or fewer, so that all have the same
-// number of shares but for one.
-unsigned even_grid(int64_t need, int64_t resident) {
-  const int64_t rounds = (need + resident - 1) / resident;
-  return (unsigned)((need + rounds - 1) / rounds);
-}
+
 int resident_groups(const void* kernel, int threads) {
   int n = 0;
   if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != hipSuccess || n < 1)
@@ -657,27 +644,24 @@ int resident_groups(const void* kernel, int threads) {
   return n * kCus;
 }
 
-template <class T, int V, int TPR, int K, bool EVEN, int ACT>
+template <class T, int V, int TPR, int K, bool EVEN, int ACT, bool STREAM>
 void forward_launch(NormArgs a, hipStream_t st) {
   constexpr int NT = forward_threads<TPR>(), RPB = NT / TPR;
-  const void* kernel = (const void*)layer_norm_forward_kernel<T, V, TPR, K, EVEN, ACT>;
+  const void* kernel = (const void*)layer_norm_forward_kernel<T, V, TPR, K, EVEN, ACT, STREAM>;
   static const int resident = resident_groups(kernel, NT);
   void* args[] = {&a};
   launch(kernel, even_grid((a.rows + RPB - 1) / RPB, resident), NT, args, st);
 }
 template <class T, int V, int TPR, int K, int ACT>
 void forward_rows(const NormArgs& a, hipStream_t st) {
-  a.cols == TPR * K * V ? forward_launch<T, V, TPR, K, true, ACT>(a, st) : forward_launch<T, V, TPR, K, false, ACT>(a, st);
+  const bool even = a.cols == TPR * K * V;
+  if constexpr (TPR >= 16) {
+    if (beyond_caches<T>(a))
+      return even ? forward_launch<T, V, TPR, K, true, ACT, true>(a, st) : forward_launch<T, V, TPR, K, false, ACT, true>(a, st);
+  }
+  even ? forward_launch<T, V, TPR, K, true, ACT, false>(a, st) : forward_launch<T, V, TPR, K, false, ACT, false>(a, st);
 }
 
-// The widest rows that a workgroup's registers hold, forward
-constexpr int kForwardCols = 16384;
-
-template <class T>
-int chunk_count(int cols) {
-  constexpr int V = 16 / sizeof(T);
-  return (cols + chunk_cols<V>() - 1) / chunk_cols<V>();
-}
 
 template <class T, int ACT>
 void run_forward(NormArgs a, hipStream_t st) {
@@ -695,45 +679,25 @@ void run_forward(NormArgs a, hipStream_t st) {
   if (a.cols <= 4096) return forward_rows<T, V, 256, K, ACT>(a, st);
   if (a.cols <= 8192) return forward_rows<T, V, 512, K, ACT>(a, st);
   if (a.cols <= kForwardCols) return forward_rows<T, V, 1024, K, ACT>(a, st);
-  a.chunks = chunk_count<T>(a.cols);
+  a.chunks = chunks_of_row(a.cols, V);
   const int64_t items = a.rows * a.chunks;
   const unsigned grid = (unsigned)(items < 1 << 20 ? items : 1 << 20);
   void* args[] = {&a};
   launch((const void*)layer_norm_chunk_statistics_kernel<T, V>, grid, kThreads, args, st);
   launch((const void*)layer_norm_chunk_forward_kernel<T, V, ACT>, grid, kThreads, args, st);
 }
-// Workgroups of the backward kernels, i.e. rows of partial sums
-struct BackwardPlan {
-  int tpr;     // threads to a row; 0: rows in chunks
-  int chunks;  // of a row
-  int64_t groups;
-};
-constexpr int kBackwardCols = 8192;
-
-BackwardPlan backward_plan(const rbl_layer_norm_shape& s) {
-  BackwardPlan p{};
-  if (s.cols <= kBackwardCols) {
-    p.tpr = s.cols <= 32 ? 4 : 8;
-    while (p.tpr < 512 && p.tpr * 8 < s.cols) p.tpr *= 2;
-    const int nt = backward_threads(p.tpr);
-    const int64_t need = (s.rows * p.tpr + nt - 1) / nt;
-    p.groups = need == 0 ? 0 : even_grid(need, (int64_t)kCus * kBackwardWaves * 64 / nt);
-  } else {
-    const int chunk = kThreads * kChunkK * (s.dtype == RBL_F32 ? 4 : 8);
-    p.chunks = (int)((s.cols + chunk - 1) / chunk);
-    const int64_t most = (kCus + p.chunks - 1) / p.chunks;
-    p.groups = s.rows < most ? s.rows : most;
-  }
-  return p;
-}
-
 template <class T, int V, int TPR, int K, int ACT>
 void backward_rows(NormArgs a, const BackwardPlan& p, bool sums, hipStream_t st) {
   const bool even = a.cols == TPR * K * V;
-  const void* kernel = sums ? even ? (const void*)layer_norm_backward_kernel<T, V, TPR, K, true, ACT, true>
-                                   : (const void*)layer_norm_backward_kernel<T, V, TPR, K, false, ACT, true>
-                       : even ? (const void*)layer_norm_backward_kernel<T, V, TPR, K, true, ACT, false>
-                              : (const void*)layer_norm_backward_kernel<T, V, TPR, K, false, ACT, false>;
+  const void* kernel = sums ? even ? (const void*)layer_norm_backward_kernel<T, V, TPR, K, true, ACT, true, false>
+                                   : (const void*)layer_norm_backward_kernel<T, V, TPR, K, false, ACT, true, false>
+                       : even ? (const void*)layer_norm_backward_kernel<T, V, TPR, K, true, ACT, false, false>
+                              : (const void*)layer_norm_backward_kernel<T, V, TPR, K, false, ACT, false, false>;
+  if constexpr (TPR >= 16) {
+    if (sums && beyond_caches<T>(a))
+      kernel = even ? (const void*)layer_norm_backward_kernel<T, V, TPR, K, true, ACT, true, true>
+                    : (const void*)layer_norm_backward_kernel<T, V, TPR, K, false, ACT, true, true>;
+  }
   void* args[] = {&a};
   launch(kernel, (unsigned)p.groups, backward_threads(TPR), args, st);
 }
@@ -778,122 +742,15 @@ void run_backward(NormArgs a, const BackwardPlan& p, hipStream_t st) {
   }
 }
 
-void check(const rbl_layer_norm_shape* s) {
-  if (!s) throw std::runtime_error("layer norm: shape is null");
-  if (s->rows < 0) throw std::runtime_error("layer norm: rows is negative");
-  if (s->cols < 1 || s->cols > (int64_t)1 << 30) throw std::runtime_error("layer norm: cols must be in [1, 2^30]");
-  if (s->dtype != RBL_F32 && s->dtype != RBL_F16 && s->dtype != RBL_BF16) throw std::runtime_error("layer norm: unknown dtype");
-  if (s->param_dtype != RBL_F32 && s->param_dtype != s->dtype)
-    throw std::runtime_error("layer norm: param_dtype must be f32 or dtype");
-  if (s->activation != RBL_ACT_NONE && s->activation != RBL_ACT_GELU)
-    throw std::runtime_error("layer norm: unknown activation");
-  if (s->x_stride < 0 || s->dy_stride < 0) throw std::runtime_error("layer norm: strides must not be negative");
-  if (s->rows > 0 && s->rows > ((int64_t)1 << 60) / s->cols) throw std::runtime_error("layer norm: rows x cols is too large");
-}
-
-int64_t forward_workspace(const rbl_layer_norm_shape& s) {
-  const int size = s.dtype == RBL_F32 ? 4 : 2, v = 16 / size;
-  if (s.cols <= kForwardCols) return 0;
-  const int64_t chunk = kThreads * kChunkK * v;
-  return s.rows * ((s.cols + chunk - 1) / chunk) * 2 * (int64_t)sizeof(float);
-}
-
-// row_sums of the chunks, then the partial sums
-int64_t backward_row_sums(const rbl_layer_norm_shape& s, const BackwardPlan& p) {
-  return p.tpr ? 0 : s.rows * p.chunks * 2 * (int64_t)sizeof(float);
-}
-int64_t backward_workspace(const rbl_layer_norm_shape& s) {
-  const BackwardPlan p = backward_plan(s);
-  return (backward_row_sums(s, p) + 15) / 16 * 16 + p.groups * 2 * ((s.cols + 3) / 4 * 4) * (int64_t)sizeof(float);
-}
-
-void check_workspace(int64_t need, const void* workspace, int64_t bytes) {
-  if (bytes < need || (need > 0 && !workspace))
-    throw std::runtime_error("layer norm: the workspace must hold " + std::to_string(need) + " bytes");
-}
-
-NormArgs args_of(const rbl_layer_norm_shape& s) {
-  NormArgs a{};
-  a.rows = s.rows;
-  a.x_stride = s.x_stride;
-  a.dy_stride = s.dy_stride;
-  a.cols = (int)s.cols;
-  a.inv_cols = 1.0f / (float)s.cols;
-  a.param_f32 = s.param_dtype == RBL_F32;
-  a.eps = s.eps;
-  return a;
-}
-
-template <int ACT>
-void forward_by_type(int dtype, const NormArgs& a, hipStream_t st) {
-  if (dtype == RBL_F32) run_forward<float, ACT>(a, st);
-  if (dtype == RBL_F16) run_forward<_Float16, ACT>(a, st);
-  if (dtype == RBL_BF16) run_forward<__bf16, ACT>(a, st);
-}
-template <int ACT>
-void backward_by_type(int dtype, const NormArgs& a, const BackwardPlan& p, hipStream_t st) {
-  if (dtype == RBL_F32) run_backward<float, ACT>(a, p, st);
-  if (dtype == RBL_F16) run_backward<_Float16, ACT>(a, p, st);
-  if (dtype == RBL_BF16) run_backward<__bf16, ACT>(a, p, st);
-}
-
 }  // namespace
+
+template <class T>
+void layer_norm_forward(const NormArgs& a, int activation, hipStream_t st) {
+  activation == RBL_ACT_GELU ? run_forward<T, RBL_ACT_GELU>(a, st) : run_forward<T, RBL_ACT_NONE>(a, st);
+}
+template <class T>
+void layer_norm_backward(const NormArgs& a, const BackwardPlan& p, int activation, hipStream_t st) {
+  activation == RBL_ACT_GELU ? run_backward<T, RBL_ACT_GELU>(a, p, st) : run_backward<T, RBL_ACT_NONE>(a, p, st);
+}
+
 }  // namespace rbl
-
-extern "C" {
-
-int64_t rbl_layer_norm_workspace(const rbl_layer_norm_shape* s, int backward) {
-  int64_t bytes = -1;
-  rbl::train_entry([&] {
-    rbl::check(s);
-    bytes = backward ? rbl::backward_workspace(*s) : rbl::forward_workspace(*s);
-  });
-  return bytes;
-}
-
-int rbl_layer_norm_forward(int device, const rbl_layer_norm_shape* s, const void* x_dev, const void* weight_dev,
-                           const void* bias_dev, void* y_dev, float* stats_dev, void* workspace_dev, int64_t workspace_bytes,
-                           void* stream) {
-  return rbl::train_entry([&] {
-    rbl::check(s);
-    if (s->rows > 0 && (!x_dev || !y_dev)) throw std::runtime_error("layer norm: x or y is null");
-    rbl::NormArgs a = rbl::args_of(*s);
-    a.x = x_dev;
-    a.w = weight_dev;
-    a.b = bias_dev;
-    a.y = y_dev;
-    a.stats = stats_dev;
-    a.partial = (float*)workspace_dev;
-    rbl::check_workspace(rbl::forward_workspace(*s), workspace_dev, workspace_bytes);
-    rbl::DeviceScope scope(device);
-    s->activation == RBL_ACT_GELU ? rbl::forward_by_type<RBL_ACT_GELU>(s->dtype, a, (hipStream_t)stream)
-                                  : rbl::forward_by_type<RBL_ACT_NONE>(s->dtype, a, (hipStream_t)stream);
-  });
-}
-
-int rbl_layer_norm_backward(int device, const rbl_layer_norm_shape* s, const void* dy_dev, const void* x_dev,
-                            const void* weight_dev, const void* bias_dev, const float* stats_dev, void* dx_dev,
-                            void* dweight_dev, void* dbias_dev, void* workspace_dev, int64_t workspace_bytes, void* stream) {
-  return rbl::train_entry([&] {
-    rbl::check(s);
-    if (s->rows > 0 && (!x_dev || !dy_dev || !stats_dev)) throw std::runtime_error("layer norm: x, dy or stats is null");
-    rbl::NormArgs a = rbl::args_of(*s);
-    a.x = x_dev;
-    a.dy = dy_dev;
-    a.w = weight_dev;
-    a.b = bias_dev;
-    a.stats = const_cast<float*>(stats_dev);
-    a.dx = dx_dev;
-    a.dw = dweight_dev;
-    a.db = dbias_dev;
-    rbl::check_workspace(rbl::backward_workspace(*s), workspace_dev, workspace_bytes);
-    const rbl::BackwardPlan p = rbl::backward_plan(*s);
-    a.row_sums = (float*)workspace_dev;
-    a.partial = a.row_sums + (rbl::backward_row_sums(*s, p) + 15) / 16 * 4;
-    rbl::DeviceScope scope(device);
-    s->activation == RBL_ACT_GELU ? rbl::backward_by_type<RBL_ACT_GELU>(s->dtype, a, p, (hipStream_t)stream)
-                                  : rbl::backward_by_type<RBL_ACT_NONE>(s->dtype, a, p, (hipStream_t)stream);
-  });
-}
-
-}  // extern "C"

@@ -730,13 +730,14 @@ def test_train_kernels_have_neither_scratch_nor_flat_loads(tmp_path):
     if not os.path.exists(hipcc):
         pytest.skip("no hipcc")
     csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "rebel_amd", "csrc")
-    for src in ("layer_norm_kernel.hip", "grad_norm_kernel.hip"):
-        out = tmp_path / (src + ".s")
-        r = subprocess.run([hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-I../../include", "-Wno-unused-result", "-Xclang",
-                            "-target-feature", "-Xclang", "-packed-fp32-ops", "-S", "--cuda-device-only", src, "-o", str(out)], cwd=csrc,
-                           stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=900)
-        assert r.returncode == 0, r.stdout[-3000:]
-        text = out.read_text()
+    srcs = ["layer_norm_f32.hip", "layer_norm_f16.hip", "layer_norm_bf16.hip", "grad_norm_kernel.hip"]
+    runs = [subprocess.Popen([hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-I../../include", "-Wno-unused-result", "-Xclang",
+                              "-target-feature", "-Xclang", "-packed-fp32-ops", "-S", "--cuda-device-only", src, "-o", str(tmp_path / src)],
+                             cwd=csrc, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) for src in srcs]
+    for src, r in zip(srcs, runs):
+        said, _ = r.communicate(timeout=900)
+        assert r.returncode == 0, said[-3000:]
+        text = (tmp_path / src).read_text()
         for word in ("flat_load", "flat_store", "scratch_load", "scratch_store", "v_pk_fma_f32", "v_pk_mul_f32", "v_pk_add_f32"):
             assert word not in text, (src, word)
         assert ".private_segment_fixed_size: 0" in text
