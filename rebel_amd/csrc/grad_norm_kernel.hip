@@ -228,24 +228,23 @@ const void* norm_kernel(int norm) {
 
 int64_t size_of(const rbl_grad& g) { return g.dtype == RBL_F32 ? 4 : 2; }
 
-int64_t chunk_size(const rbl_grad* grads, int n) {
-  int64_t all = 0;
-  for (int i = 0; i < n; ++i) all += grads[i].numel * size_of(grads[i]);
-  int64_t chunk = std::min(all / kChunksResident, kChunkFull);
-  chunk = std::max({chunk, all / kChunksMost, kChunkMin});
-  return (chunk + kChunkMin - 1) / kChunkMin * kChunkMin;
-}
+struct Plan {
+  int shift;  // a chunk has 2^shift bytes
+  int total;  // chunks
+};
+int64_t chunks_of(const rbl_grad& g, int shift) { return (g.numel * size_of(g) + ((int64_t)1 << shift) - 1) >> shift; }
 
-int64_t chunks_of(const rbl_grad& g, int64_t chunk) { return (g.numel * size_of(g) + chunk - 1) / chunk; }
-int64_t chunk_count(const rbl_grad* grads, int n, int64_t chunk) {
-  int64_t all = 0;
-  for (int i = 0; i < n; ++i) all += chunks_of(grads[i], chunk);
-  return all;
+Plan plan_of(const rbl_grad* grads, int n) {
+  int64_t all = 0, chunks = 0;
+  for (int i = 0; i < n; ++i) all += grads[i].numel * size_of(grads[i]);
+  const int64_t chunk = std::max({std::min(all / kChunksResident, kChunkFull), all / kChunksMost, kChunkMin});
+  Plan p{0, 0};
+  while ((int64_t)1 << p.shift < chunk) ++p.shift;
+  for (int i = 0; i < n; ++i) chunks += chunks_of(grads[i], p.shift);
+  p.total = (int)chunks;
+  return p;
 }
-int64_t workspace_size(const rbl_grad* grads, int n) {
-  const int64_t chunks = chunk_count(grads, n, chunk_size(grads, n));
-  return chunks ? 8 * (chunks + 1) : 0;
-}
+int64_t workspace_size(const Plan& p) { return p.total ? 8 * ((int64_t)p.total + 1) : 0; }
 
 void check(const rbl_grad* grads, int n) {
   if (n < 0) throw std::runtime_error("gradients: n is negative");
@@ -263,8 +262,8 @@ void check_norm(int norm) {
   if (norm != RBL_NORM_1 && norm != RBL_NORM_2 && norm != RBL_NORM_INF)
     throw std::runtime_error("gradients: the norm must be 1, 2 or infinity");
 }
-void check_workspace(const rbl_grad* grads, int n, const void* workspace, int64_t bytes) {
-  const int64_t need = workspace_size(grads, n);
+void check_workspace(const Plan& p, const void* workspace, int64_t bytes) {
+  const int64_t need = workspace_size(p);
   if (bytes < need || (need > 0 && !workspace))
     throw std::runtime_error("gradients: the workspace must hold " + std::to_string(need) + " bytes");
 }
@@ -273,9 +272,9 @@ void check_bound(double max_norm) {
 }
 
 // One launch of `kernel` for every table of tensors; `backwards`: the last table first
-void for_tables(const void* kernel, const rbl_grad* grads, int n, ClipArgs a, bool backwards, hipStream_t st) {
-  a.chunk = (int)chunk_size(grads, n);
-  a.total = (int)chunk_count(grads, n, a.chunk);
+void for_tables(const void* kernel, const rbl_grad* grads, int n, ClipArgs a, const Plan& p, bool backwards, hipStream_t st) {
+  a.chunk = 1 << p.shift;
+  a.total = p.total;
   GradTable t;
   int from = 0, to = n, first = backwards ? a.total : 0;
   while (from < to) {
@@ -291,7 +290,7 @@ void for_tables(const void* kernel, const rbl_grad* grads, int n, ClipArgs a, bo
     count = 0;
     for (int i = lo; i < hi; ++i) {
       if (grads[i].numel == 0) continue;
-      const int64_t whole = chunks_of(grads[i], a.chunk);
+      const int64_t whole = chunks_of(grads[i], p.shift);
       t.data[count] = grads[i].data_dev;
       t.first_chunk[count] = chunks;
       t.last[count] = (unsigned)(grads[i].numel - (whole - 1) * (a.chunk / size_of(grads[i]))) | (unsigned)grads[i].dtype << kTypeShift;
@@ -319,7 +318,7 @@ int64_t rbl_grad_workspace(const rbl_grad* grads, int n) {
   int64_t bytes = -1;
   rbl::train_entry([&] {
     rbl::check(grads, n);
-    bytes = rbl::workspace_size(grads, n);
+    bytes = rbl::workspace_size(rbl::plan_of(grads, n));
   });
   return bytes;
 }
@@ -329,14 +328,15 @@ int rbl_grad_norm(int device, const rbl_grad* grads, int n, int norm, float* nor
   return rbl::train_entry([&] {
     rbl::check(grads, n);
     rbl::check_norm(norm);
-    rbl::check_workspace(grads, n, workspace_dev, workspace_bytes);
+    const rbl::Plan p = rbl::plan_of(grads, n);
+    rbl::check_workspace(p, workspace_dev, workspace_bytes);
     if (!norm_dev) throw std::runtime_error("gradients: norm_dev is null");
     rbl::DeviceScope scope(device);
     rbl::ClipArgs a{};
     a.sums = (double*)workspace_dev;
     a.norm_out = norm_dev;
-    rbl::for_tables(rbl::sums_kernel(norm), grads, n, a, false, (hipStream_t)stream);
-    a.total = (int)rbl::chunk_count(grads, n, rbl::chunk_size(grads, n));
+    rbl::for_tables(rbl::sums_kernel(norm), grads, n, a, p, false, (hipStream_t)stream);
+    a.total = p.total;
     void* args[] = {&a};
     rbl::launch(rbl::norm_kernel(norm), 1, rbl::kNormThreads, args, (hipStream_t)stream);
   });
@@ -348,20 +348,21 @@ int rbl_grad_clip(int device, const rbl_grad* grads, int n, int norm, double max
     rbl::check(grads, n);
     rbl::check_norm(norm);
     rbl::check_bound(max_norm);
-    rbl::check_workspace(grads, n, workspace_dev, workspace_bytes);
+    const rbl::Plan p = rbl::plan_of(grads, n);
+    rbl::check_workspace(p, workspace_dev, workspace_bytes);
     if (!norm_dev) throw std::runtime_error("gradients: norm_dev is null");
     rbl::DeviceScope scope(device);
     rbl::ClipArgs a{};
     a.sums = (double*)workspace_dev;
     a.norm_out = norm_dev;
     a.max_norm = max_norm;
-    rbl::for_tables(rbl::sums_kernel(norm), grads, n, a, false, (hipStream_t)stream);
-    a.total = (int)rbl::chunk_count(grads, n, rbl::chunk_size(grads, n));
+    rbl::for_tables(rbl::sums_kernel(norm), grads, n, a, p, false, (hipStream_t)stream);
+    a.total = p.total;
     if (a.total == 0 || a.total > rbl::kSumsMost) {  // nothing to scale: the norm of nothing
       void* args[] = {&a};
       rbl::launch(rbl::norm_kernel(norm), 1, rbl::kNormThreads, args, (hipStream_t)stream);
     }
-    rbl::for_tables(rbl::scale_kernel(norm), grads, n, a, true, (hipStream_t)stream);
+    rbl::for_tables(rbl::scale_kernel(norm), grads, n, a, p, true, (hipStream_t)stream);
   });
 }
 
@@ -374,7 +375,7 @@ int rbl_grad_scale(int device, const rbl_grad* grads, int n, double max_norm, co
     rbl::ClipArgs a{};
     a.norm_in = norm_dev;
     a.max_norm = max_norm;
-    rbl::for_tables((const void*)rbl::grad_scale_kernel<0>, grads, n, a, true, (hipStream_t)stream);
+    rbl::for_tables((const void*)rbl::grad_scale_kernel<0>, grads, n, a, rbl::plan_of(grads, n), true, (hipStream_t)stream);
   });
 }
 

@@ -202,10 +202,16 @@ struct Gradients {
   Tensor any;
 };
 
-Gradients gather(const std::vector<Tensor>& tensors, bool scaled) {
+Gradients gather(const std::vector<const Tensor*>& tensors, bool scaled) {
   Gradients g;
-  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
-  for (const Tensor& t : tensors) {
+  g.list.reserve(tensors.size());
+  struct Span {
+    uintptr_t begin, end;
+  };
+  std::vector<Span> spans;
+  if (scaled) spans.reserve(tensors.size());
+  for (const Tensor* each : tensors) {
+    const Tensor& t = *each;
     require(t.defined(), "gradients: a tensor is undefined");
     require(t.layout() == at::kStrided, "gradients: sparse gradients are not supported");
     const int type = element_type(t.scalar_type());
@@ -213,9 +219,11 @@ Gradients gather(const std::vector<Tensor>& tensors, bool scaled) {
     if (!g.any.defined()) g.any = t;
     require(t.device() == g.any.device(), "gradients: all must be on one device, not on ", g.any.device(), " and ", t.device());
     if (t.numel() == 0) continue;
-    Tensor dense = t;
+    void* at_data = t.data_ptr();
     if (!t.is_non_overlapping_and_dense()) {
-      dense = t.contiguous();
+      const Tensor dense = t.contiguous();  // alive until the launch
+      at_data = dense.data_ptr();
+      g.copies.emplace_back(t, dense);
       if (scaled) {
         // the furthest element; no two may share their memory
         int64_t reach = 1;
@@ -223,20 +231,18 @@ Gradients gather(const std::vector<Tensor>& tensors, bool scaled) {
           require(t.size(i) == 1 || t.stride(i) != 0, "gradients: a tensor that repeats its memory cannot be scaled in place");
           reach += (t.size(i) - 1) * t.stride(i);
         }
-        g.copies.emplace_back(t, dense);
         const auto at = (uintptr_t)t.data_ptr();
-        spans.emplace_back(at, at + reach * t.element_size());
+        spans.push_back({at, at + reach * t.element_size()});
       }
     } else if (scaled) {
-      const auto at = (uintptr_t)t.data_ptr();
-      spans.emplace_back(at, at + t.numel() * t.element_size());
+      const auto at = (uintptr_t)at_data;
+      spans.push_back({at, at + t.numel() * t.element_size()});
     }
-    g.list.push_back({dense.data_ptr(), dense.numel(), type});
-    if (!scaled && dense.data_ptr() != t.data_ptr()) g.copies.emplace_back(t, dense);  // alive until the launch
+    g.list.push_back({at_data, t.numel(), type});
   }
-  std::sort(spans.begin(), spans.end());
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
   for (size_t i = 1; i < spans.size(); ++i)
-    require(spans[i].first >= spans[i - 1].second, "gradients: two of them share memory (the same tensor twice?)");
+    require(spans[i].begin >= spans[i - 1].end, "gradients: two of them share memory (the same tensor twice?)");
   if (g.any.defined()) require(g.any.is_cuda(), "gradients: must be on the GPU: there is no CPU path");
   return g;
 }
@@ -257,31 +263,51 @@ Tensor norm_of(const Gradients& g, int kind) {
   return norm;
 }
 
-Tensor grad_norm(const std::vector<Tensor>& tensors, double norm_type) {
+// The tensors of a Python list, by reference: the list holds them, and the interpreter stays locked.
+std::vector<const Tensor*> tensors_of(const py::list& list) {
+  std::vector<const Tensor*> out;
+  out.reserve(list.size());
+  for (const py::handle h : list) {
+    if (!THPVariable_Check(h.ptr()))
+      throw py::type_error("gradients: expected tensors, not " + std::string(Py_TYPE(h.ptr())->tp_name));
+    out.push_back(&THPVariable_Unpack(h.ptr()));
+  }
+  return out;
+}
+
+Tensor grad_norm(const py::list& tensors, double norm_type) {
   at::NoGradGuard no_grad;
   const int kind = norm_kind(norm_type);
-  const Gradients g = gather(tensors, false);
+  const Gradients g = gather(tensors_of(tensors), false);
   return g.any.defined() ? norm_of(g, kind) : at::zeros({});
 }
 
-Tensor clip_grad_norm(const std::vector<Tensor>& parameters, double max_norm, double norm_type, bool error_if_nonfinite) {
+Tensor clip_grad_norm(const py::list& parameters, double max_norm, double norm_type, bool error_if_nonfinite) {
   at::NoGradGuard no_grad;
   const int kind = norm_kind(norm_type);
   require(max_norm >= 0, "gradients: max_norm must be a number >= 0, not ", max_norm);
-  std::vector<Tensor> grads;
+  std::vector<const Tensor*> grads;
   grads.reserve(parameters.size());
-  for (const Tensor& p : parameters)
-    if (p.grad().defined()) grads.push_back(p.grad());
+  for (const Tensor* p : tensors_of(parameters)) {
+    const Tensor& grad = p->grad();
+    if (grad.defined()) grads.push_back(&grad);
+  }
   const Gradients g = gather(grads, true);
   if (!g.any.defined()) return at::zeros({});
   c10::DeviceGuard guard(g.any.device());
   const int n = (int)g.list.size();
   Tensor norm;
+  std::vector<Tensor> held;  // while other threads may run and give the parameters other gradients
   if (error_if_nonfinite) {
     require(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
                 "gradients: error_if_nonfinite looks at the norm on the host, which a capture cannot do");
     norm = norm_of(g, kind);
-    const float value = norm.item<float>();
+    float value;
+    {
+      for (const Tensor* t : grads) held.push_back(*t);
+      py::gil_scoped_release unlocked;
+      value = norm.item<float>();
+    }
     if (!std::isfinite(value))
       throw std::runtime_error(c10::str("gradients: the total norm of order ", norm_type, " is ", value,
                                         ", so they were not clipped (error_if_nonfinite)"));
@@ -301,7 +327,7 @@ Tensor clip_grad_norm(const std::vector<Tensor>& parameters, double max_norm, do
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_norm", &layer_norm, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("eps"), py::arg("activation"),
         py::call_guard<py::gil_scoped_release>());
-  m.def("grad_norm", &grad_norm, py::arg("tensors"), py::arg("norm_type"), py::call_guard<py::gil_scoped_release>());
+  m.def("grad_norm", &grad_norm, py::arg("tensors"), py::arg("norm_type"));
   m.def("clip_grad_norm", &clip_grad_norm, py::arg("parameters"), py::arg("max_norm"), py::arg("norm_type"),
-        py::arg("error_if_nonfinite"), py::call_guard<py::gil_scoped_release>());
+        py::arg("error_if_nonfinite"));
 }

@@ -647,6 +647,9 @@ def test_clipping_refuses():
                        (lambda: training.grad_norm([a.grad, a.grad.to("meta")]), "one device")):
         with pytest.raises(ValueError, match=word):
             call()
+    for call in (lambda: training.grad_norm([a.grad, None]), lambda: training.clip_grad_norm_([a, 3.0], 1.0)):
+        with pytest.raises(TypeError, match="expected tensors"):
+            call()
     b = torch.nn.Parameter(torch.zeros(4))
     b.grad = a.grad
     with pytest.raises(ValueError, match="share memory"):
