@@ -21,7 +21,7 @@ struct NormArgs {
 };
 
 // The widest rows that a workgroup's registers hold, forward
-constexpr int kForwardCols = 16384;
+constexpr int kForwardCols = 32768;
 
 // Longer ones go in chunks of kChunkK vectors to each of kThreads threads.
 constexpr int kThreads = 256, kChunkK = 4;
@@ -47,21 +47,28 @@ struct BackwardPlan {
   int tpr;     // threads to a row; 0: rows in chunks
   int chunks;  // of a row
   int64_t groups;
+  bool few;  // so few rows that the parameters' gradients are taken from x and dy in the same launch
 };
-constexpr int kBackwardCols = 8192;
+constexpr int kBackwardCols = 16384;
+
+// Few rows: 512 x 256 f32 + GELU takes 5.0 us in one launch (5.9 with partial sums), 512 x 4096 11.7 (13.2), 24 x 65537 14 (20); with
+// more of them the second reading costs more than it saves (1024 x 256 7.6 (6.3), 512 x 8192 22.9 (17.2)).
+constexpr int64_t kFewRows = 512, kFewElements = 1 << 21;
 
 inline BackwardPlan backward_plan(const rbl_layer_norm_shape& s) {
   BackwardPlan p{};
+  p.few = s.rows <= kFewRows && s.rows * s.cols <= kFewElements;
   if (s.cols <= kBackwardCols) {
     p.tpr = s.cols <= 32 ? 4 : 8;
     while (p.tpr < 512 && p.tpr * 8 < s.cols) p.tpr *= 2;
+    if (s.cols > 8192) p.tpr = 1024;
     const int nt = backward_threads(p.tpr);
     const int64_t need = (s.rows * p.tpr + nt - 1) / nt;
-    p.groups = need == 0 ? 0 : even_grid(need, (int64_t)kCus * kBackwardWaves * 64 / nt);
+    p.groups = p.few || need == 0 ? need : even_grid(need, (int64_t)kCus * (nt > kBackwardWaves * 64 ? 1 : kBackwardWaves * 64 / nt));
   } else {
     p.chunks = chunks_of_row(s.cols, s.dtype == RBL_F32 ? 4 : 8);
-    const int64_t most = (kCus + p.chunks - 1) / p.chunks;
-    p.groups = s.rows < most ? s.rows : most;
+    const int64_t most = (2 * kCus + p.chunks - 1) / p.chunks;  // eight wavefronts to a CU here too
+    p.groups = p.few || s.rows < most ? s.rows : most;
   }
   return p;
 }

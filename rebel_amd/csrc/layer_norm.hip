@@ -28,7 +28,7 @@ int64_t backward_row_sums(const rbl_layer_norm_shape& s, const BackwardPlan& p) 
 }
 int64_t backward_workspace(const rbl_layer_norm_shape& s) {
   const BackwardPlan p = backward_plan(s);
-  return (backward_row_sums(s, p) + 15) / 16 * 16 + p.groups * 2 * ((s.cols + 3) / 4 * 4) * (int64_t)sizeof(float);
+  return (backward_row_sums(s, p) + 15) / 16 * 16 + (p.few ? 0 : p.groups) * 2 * ((s.cols + 3) / 4 * 4) * (int64_t)sizeof(float);
 }
 
 void check_workspace(int64_t need, const void* workspace, int64_t bytes) {

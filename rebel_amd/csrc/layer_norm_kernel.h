@@ -11,6 +11,8 @@
 // The element types are compiled apart (layer_norm_f32.hip, layer_norm_f16.hip, layer_norm_bf16.hip); layer_norm.hip holds the C
 // entries.
 #pragma once
+#include <algorithm>
+
 #include "layer_norm.h"
 
 namespace rbl {
@@ -77,13 +79,14 @@ struct Pack {
 template <int V, int TPR, int K, bool EVEN>
 struct Place {
   int col, skip;
+  static __device__ __forceinline__ constexpr bool whole(int k) { return EVEN || (TPR >= 8 && 2 * k + 2 <= K); }
   Place() = default;
   __device__ __forceinline__ Place(int t, int k, int cols) {
     const int at = (t + k * TPR) * V;
-    col = EVEN || at + V <= cols ? at : cols - V;
-    skip = EVEN ? 0 : at - col;
+    col = whole(k) || at + V <= cols ? at : cols - V;
+    skip = whole(k) ? 0 : at - col;
   }
-  __device__ __forceinline__ bool owns(int k, int i) const { return EVEN || (TPR >= 8 && 2 * k + 2 <= K) || i >= skip; }
+  __device__ __forceinline__ bool owns(int k, int i) const { return whole(k) || i >= skip; }
 };
 
 // Stores the elements that a thread owns.  A moved-back vector stores its own alone: what it has computed for its neighbour's
@@ -218,22 +221,28 @@ __global__ __launch_bounds__(forward_threads<TPR>()) void layer_norm_forward_ker
       load_params<T, V>(a, a.b, at[k].col, 0.0f, b[k]);
     }
   }
+  constexpr bool AHEAD = K * V <= 16;  // the next row is on its way while one is computed
   vec next[K];
-  load_row<T, V, STREAM>(next, a.x, row * a.x_stride, at);
+  if (AHEAD) load_row<T, V, STREAM>(next, a.x, row * a.x_stride, at);
   for (; row < a.rows; row += step) {
+    if (!AHEAD) load_row<T, V, STREAM>(next, a.x, row * a.x_stride, at);
     float x[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) x[k][i] = (float)next[k][i];
-    const int64_t ahead = row + step < a.rows ? row + step : row;  // the next row is on its way while this one is computed
-    load_row<T, V, STREAM>(next, a.x, ahead * a.x_stride, at);
+      for (int i = 0; i < V; ++i) {
+        x[k][i] = (float)next[k][i];
+        if (!AHEAD) asm("" : "+v"(x[k][i]));  // not both the packed and the unpacked row: there is no room
+      }
+    const int64_t ahead = row + step < a.rows ? row + step : row;
+    if (AHEAD) load_row<T, V, STREAM>(next, a.x, ahead * a.x_stride, at);
     float mean, r;
     statistics<V, TPR, K, EVEN>(x, at, a.inv_cols, a.eps, slots, turn, mean, r);
     T* y = (T*)a.y + row * a.cols;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (!KEEP) {
+        __builtin_amdgcn_sched_barrier(0);  // not all of the parameters at once: they would spill
         load_params<T, V>(a, a.w, at[k].col, 1.0f, w[k]);
         load_params<T, V>(a, a.b, at[k].col, 0.0f, b[k]);
       }
@@ -356,20 +365,24 @@ __device__ __forceinline__ void put_sums(float* out, const float (&v)[V], int sk
 }
 
 // Backward, a row in the registers of TPR threads: x and dy are read once, dx is written, and (SUMS) g h and g are summed up over
-// the rows of the workgroup, in registers; the workgroups' sums are joined by layer_norm_sums_kernel.
+// the rows of the workgroup, in registers (rows of 1024 threads: in LDS, each thread its own 16-byte cells); the workgroups' sums
+// are joined by layer_norm_sums_kernel.  Workgroup `group` of `groups`.
 template <class T, int V, int TPR, int K, bool EVEN, int ACT, bool SUMS, bool STREAM>
-__global__ __launch_bounds__(backward_threads(TPR)) void layer_norm_backward_kernel(NormArgs a) {
+__device__ __forceinline__ void backward_of_rows(const NormArgs& a, int group, int groups) {
   constexpr int NT = backward_threads(TPR), RPB = NT / TPR;
   typedef typename Pack<T, V>::type vec;
   __shared__ float slots[TPR > 64 ? 4 * TPR / 64 : 1];
   __shared__ float joined[SUMS && TPR <= 64 ? 2 * TPR * K * V : 1];
+  constexpr bool CELLS = SUMS && TPR == 1024;
+  typedef float cell __attribute__((ext_vector_type(4)));
+  __shared__ cell cells[CELLS ? 2 * K * V / 4 * TPR : 1];
   int turn = 0;
   const int t = threadIdx.x % TPR;
   Place<V, TPR, K, EVEN> at[K];
-  const int64_t step = (int64_t)gridDim.x * RPB;
-  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-  constexpr bool KEEP = K * V <= 16;
-  float w[K][V], b[K][V], dw[K][V], db[K][V];
+  const int64_t step = (int64_t)groups * RPB;
+  int64_t row = (int64_t)group * RPB + threadIdx.x / TPR;
+  constexpr bool KEEP = K * V <= 16 && TPR < 1024;
+  float w[K][V], b[K][V], dw[CELLS ? 1 : K][V], db[CELLS ? 1 : K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     at[k] = Place<V, TPR, K, EVEN>(t, k, a.cols);
@@ -377,15 +390,28 @@ __global__ __launch_bounds__(backward_threads(TPR)) void layer_norm_backward_ker
       load_params<T, V>(a, a.w, at[k].col, 1.0f, w[k]);
       if (ACT != RBL_ACT_NONE) load_params<T, V>(a, a.b, at[k].col, 0.0f, b[k]);
     }
+    if constexpr (CELLS) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0;
+      for (int i = 0; i < V / 4; ++i)
+        cells[(k * V / 4 + i) * TPR + t] = cells[((K + k) * V / 4 + i) * TPR + t] = cell{0, 0, 0, 0};
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0;
+    }
   }
   if (row < a.rows) {
     vec next_x[K], next_dy[K];
     float2 next_s = *(const float2*)(a.stats + 2 * row);
-    load_row<T, V, STREAM>(next_x, a.x, row * a.x_stride, at);
-    load_row<T, V, STREAM>(next_dy, a.dy, row * a.dy_stride, at);
+    constexpr bool AHEAD = TPR < 1024;  // the next row is on its way while one is computed
+    if (AHEAD) {
+      load_row<T, V, STREAM>(next_x, a.x, row * a.x_stride, at);
+      load_row<T, V, STREAM>(next_dy, a.dy, row * a.dy_stride, at);
+    }
     for (; row < a.rows; row += step) {
+      if (!AHEAD) {
+        load_row<T, V, STREAM>(next_x, a.x, row * a.x_stride, at);
+        load_row<T, V, STREAM>(next_dy, a.dy, row * a.dy_stride, at);
+      }
       const float mean = next_s.x, r = next_s.y;
       float h[K][V], g[K][V];
 #pragma unroll
@@ -397,22 +423,42 @@ __global__ __launch_bounds__(backward_threads(TPR)) void layer_norm_backward_ker
         }
       const int64_t ahead = row + step < a.rows ? row + step : row;
       next_s = *(const float2*)(a.stats + 2 * ahead);
-      load_row<T, V, STREAM>(next_x, a.x, ahead * a.x_stride, at);
-      load_row<T, V, STREAM>(next_dy, a.dy, ahead * a.dy_stride, at);
+      if (AHEAD) {
+        load_row<T, V, STREAM>(next_x, a.x, ahead * a.x_stride, at);
+        load_row<T, V, STREAM>(next_dy, a.dy, ahead * a.dy_stride, at);
+      }
       float s[2] = {0, 0};
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (!KEEP) {
+          __builtin_amdgcn_sched_barrier(0);
           load_params<T, V>(a, a.w, at[k].col, 1.0f, w[k]);
           if (ACT != RBL_ACT_NONE) load_params<T, V>(a, a.b, at[k].col, 0.0f, b[k]);
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           if (ACT != RBL_ACT_NONE) g[k][i] *= activate_slope<ACT>(__builtin_fmaf(h[k][i], w[k][i], b[k][i]));
-          if (SUMS) {
+          if (SUMS && !CELLS) {
             dw[k][i] = __builtin_fmaf(g[k][i], h[k][i], dw[k][i]);
             db[k][i] += g[k][i];
           }
+        }
+        if constexpr (CELLS) {
+#pragma unroll
+          for (int i = 0; i < V / 4; ++i) {
+            cell &p = cells[(k * V / 4 + i) * TPR + t], &q = cells[((K + k) * V / 4 + i) * TPR + t];
+            cell u = p, v = q;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              u[j] = __builtin_fmaf(g[k][i * 4 + j], h[k][i * 4 + j], u[j]);
+              v[j] += g[k][i * 4 + j];
+            }
+            p = u;
+            q = v;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
           g[k][i] *= w[k][i];
           s[0] += g[k][i];
           s[1] = __builtin_fmaf(g[k][i], h[k][i], s[1]);
@@ -434,8 +480,18 @@ __global__ __launch_bounds__(backward_threads(TPR)) void layer_norm_backward_ker
   }
   if constexpr (SUMS) {
     const int64_t width = (a.cols + 3) / 4 * 4;
-    float* out = a.partial + blockIdx.x * 2 * width;
-    if constexpr (TPR > 64) {
+    float* out = a.partial + group * 2 * width;
+    if constexpr (CELLS) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+          float v[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[i] = cells[((which * K + k) * V / 4 + i / 4) * TPR + t][i % 4];
+          put_sums<V, EVEN>(out + which * width + at[k].col, v, at[k].skip);
+        }
+    } else if constexpr (TPR > 64) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         put_sums<V, EVEN>(out + at[k].col, dw[k], at[k].skip);
@@ -453,15 +509,15 @@ __global__ __launch_bounds__(backward_threads(TPR)) void layer_norm_backward_ker
             dw[k][i] += __shfl_xor(dw[k][i], d);
             db[k][i] += __shfl_xor(db[k][i], d);
           }
-      for (int group = 0; group < GROUPS; ++group) {
-        if ((int)threadIdx.x / 64 == group && threadIdx.x % 64 < TPR) {
+      for (int wave = 0; wave < GROUPS; ++wave) {
+        if ((int)threadIdx.x / 64 == wave && threadIdx.x % 64 < TPR) {
 #pragma unroll
           for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
               // element i of vector v at [i][v]: consecutive lanes in consecutive banks
               float* p = joined + (k * V + i) * TPR + t;
-              if (group == 0) {
+              if (wave == 0) {
                 p[0] = dw[k][i];
                 p[TPR * K * V] = db[k][i];
               } else {
@@ -482,6 +538,88 @@ __global__ __launch_bounds__(backward_threads(TPR)) void layer_norm_backward_ker
       }
     }
   }
+}
+
+template <class T, int V, int TPR, int K, bool EVEN, int ACT, bool SUMS, bool STREAM>
+__global__ __launch_bounds__(backward_threads(TPR)) void layer_norm_backward_kernel(NormArgs a) {
+  backward_of_rows<T, V, TPR, K, EVEN, ACT, SUMS, STREAM>(a, blockIdx.x, gridDim.x);
+}
+
+// The parameters' gradients of few rows, straight from x and dy: 4 V columns to a workgroup, NT / 4 threads down the rows.  No
+// partial sums and no second launch for them, but x and dy are read a second time.
+template <class T, int V, int ACT, int NT>
+__device__ __forceinline__ void backward_of_columns(const NormArgs& a, int block) {
+  constexpr int LANES = 4, SLICES = NT / LANES, AHEAD = 4;
+  typedef typename Pack<T, V>::type vec;
+  __shared__ float part[NT / 64][2][LANES * V];
+  const int lane = threadIdx.x % LANES, slice = threadIdx.x / LANES;
+  // as in Place: the last vector is moved back to end with the row
+  const int begin = (block * LANES + lane) * V, col = begin + V <= a.cols ? begin : a.cols - V, skip = begin - col;
+  float w[V], b[V], dw[V], db[V];
+  if (ACT != RBL_ACT_NONE) {
+    load_params<T, V>(a, a.w, col, 1.0f, w);
+    load_params<T, V>(a, a.b, col, 0.0f, b);
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) dw[i] = db[i] = 0;
+  for (int64_t row = slice; row < a.rows; row += SLICES * AHEAD) {
+    vec x[AHEAD], dy[AHEAD];
+    float2 st[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {  // behind the last row: row again, and its gradient is left out
+      const int64_t r = row + k * SLICES < a.rows ? row + k * SLICES : row;
+      x[k] = *(const vec*)((const T*)a.x + r * a.x_stride + col);
+      dy[k] = *(const vec*)((const T*)a.dy + r * a.dy_stride + col);
+      st[k] = *(const float2*)(a.stats + 2 * r);
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      if (k > 0 && row + k * SLICES >= a.rows) break;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float h = ((float)x[k][i] - st[k].x) * st[k].y;
+        float g = (float)dy[k][i];
+        if (ACT != RBL_ACT_NONE) g *= activate_slope<ACT>(__builtin_fmaf(h, w[i], b[i]));
+        dw[i] = __builtin_fmaf(g, h, dw[i]);
+        db[i] += g;
+      }
+    }
+  }
+#pragma unroll
+  for (int d = LANES; d < 64; d *= 2)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      dw[i] += __shfl_xor(dw[i], d);
+      db[i] += __shfl_xor(db[i], d);
+    }
+  if (threadIdx.x % 64 < LANES) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      part[threadIdx.x / 64][0][lane * V + i] = dw[i];
+      part[threadIdx.x / 64][1][lane * V + i] = db[i];
+    }
+  }
+  lds_barrier();
+  for (int j = threadIdx.x; j < 2 * LANES * V; j += NT) {
+    const int which = j / (LANES * V), c = j % (LANES * V);
+    float v = part[0][which][c];
+#pragma unroll
+    for (int wave = 1; wave < NT / 64; ++wave) v += part[wave][which][c];
+    const int at = (block * LANES + c / V) * V, first = at + V <= a.cols ? at : a.cols - V;
+    if (c % V >= at - first) {
+      if (which == 0 && a.dw) put_param<T>(a, a.dw, first + c % V, v);
+      if (which == 1 && a.db) put_param<T>(a, a.db, first + c % V, v);
+    }
+  }
+}
+
+// Few rows, in one launch: the first `row_groups` workgroups make dx, the others the parameters' gradients.
+template <class T, int V, int TPR, int K, bool EVEN, int ACT>
+__global__ __launch_bounds__(backward_threads(TPR)) void layer_norm_backward_few_kernel(NormArgs a, int row_groups) {
+  if ((int)blockIdx.x < row_groups)
+    backward_of_rows<T, V, TPR, K, EVEN, ACT, false, false>(a, blockIdx.x, row_groups);
+  else
+    backward_of_columns<T, V, ACT, backward_threads(TPR)>(a, blockIdx.x - row_groups);
 }
 
 // The parameters' gradients from `count` rows of partial sums, each [2][width]: COLS columns to a workgroup, the other threads
@@ -565,9 +703,9 @@ __global__ __launch_bounds__(kThreads) void layer_norm_chunk_backward_sums_kerne
 
 // ... then dx, and the parameters' gradients summed up over every `slices`-th row of a chunk
 template <class T, int V, int ACT, bool SUMS>
-__global__ __launch_bounds__(kThreads) void layer_norm_chunk_backward_kernel(NormArgs a, int slices) {
+__device__ __forceinline__ void backward_of_chunk(const NormArgs& a, int block, int slices) {
   typedef typename Pack<T, V>::type vec;
-  const int chunk = blockIdx.x % a.chunks, slice = blockIdx.x / a.chunks;
+  const int chunk = block % a.chunks, slice = block / a.chunks;
   const int begin = chunk * chunk_cols<V>(), cols = min(a.cols - begin, chunk_cols<V>());
   int col[kChunkK], skip[kChunkK];
   float dw[kChunkK][V], db[kChunkK][V];
@@ -636,6 +774,19 @@ constexpr int64_t kStreamBytes = (int64_t)512 << 20;
 template <class T>
 bool beyond_caches(const NormArgs& a) { return a.rows * a.cols * (int64_t)sizeof(T) >= kStreamBytes; }
 
+template <class T, int V, int ACT, bool SUMS>
+__global__ __launch_bounds__(kThreads) void layer_norm_chunk_backward_kernel(NormArgs a, int slices) {
+  backward_of_chunk<T, V, ACT, SUMS>(a, blockIdx.x, slices);
+}
+// As layer_norm_backward_few_kernel; `slices` rows at a time.
+template <class T, int V, int ACT>
+__global__ __launch_bounds__(kThreads) void layer_norm_chunk_backward_few_kernel(NormArgs a, int slices) {
+  const int row_groups = slices * a.chunks;
+  if ((int)blockIdx.x < row_groups)
+    backward_of_chunk<T, V, ACT, false>(a, blockIdx.x, slices);
+  else
+    backward_of_columns<T, V, ACT, kThreads>(a, blockIdx.x - row_groups);
+}
 
 int resident_groups(const void* kernel, int threads) {
   int n = 0;
@@ -678,7 +829,8 @@ void run_forward(NormArgs a, hipStream_t st) {
   if (a.cols <= 2048) return forward_rows<T, V, 128, K, ACT>(a, st);
   if (a.cols <= 4096) return forward_rows<T, V, 256, K, ACT>(a, st);
   if (a.cols <= 8192) return forward_rows<T, V, 512, K, ACT>(a, st);
-  if (a.cols <= kForwardCols) return forward_rows<T, V, 1024, K, ACT>(a, st);
+  if (a.cols <= 16384) return forward_rows<T, V, 1024, K, ACT>(a, st);
+  if (a.cols <= kForwardCols) return forward_rows<T, V, 1024, 2 * K, ACT>(a, st);
   a.chunks = chunks_of_row(a.cols, V);
   const int64_t items = a.rows * a.chunks;
   const unsigned grid = (unsigned)(items < 1 << 20 ? items : 1 << 20);
@@ -686,9 +838,18 @@ void run_forward(NormArgs a, hipStream_t st) {
   launch((const void*)layer_norm_chunk_statistics_kernel<T, V>, grid, kThreads, args, st);
   launch((const void*)layer_norm_chunk_forward_kernel<T, V, ACT>, grid, kThreads, args, st);
 }
+
 template <class T, int V, int TPR, int K, int ACT>
 void backward_rows(NormArgs a, const BackwardPlan& p, bool sums, hipStream_t st) {
   const bool even = a.cols == TPR * K * V;
+  if (sums && p.few) {
+    int row_groups = a.dx ? (int)p.groups : 0;
+    void* args[] = {&a, &row_groups};
+    launch(even ? (const void*)layer_norm_backward_few_kernel<T, V, TPR, K, true, ACT>
+                : (const void*)layer_norm_backward_few_kernel<T, V, TPR, K, false, ACT>,
+           (unsigned)(row_groups + (a.cols + 4 * V - 1) / (4 * V)), backward_threads(TPR), args, st);
+    return;
+  }
   const void* kernel = sums ? even ? (const void*)layer_norm_backward_kernel<T, V, TPR, K, true, ACT, true, false>
                                    : (const void*)layer_norm_backward_kernel<T, V, TPR, K, false, ACT, true, false>
                        : even ? (const void*)layer_norm_backward_kernel<T, V, TPR, K, true, ACT, false, false>
@@ -718,21 +879,25 @@ void run_backward(NormArgs a, const BackwardPlan& p, hipStream_t st) {
     else if (p.tpr == 256) backward_rows<T, V, 256, K, ACT>(a, p, sums, st);
     else if (p.tpr == 512 && a.cols <= 4096) backward_rows<T, V, 512, K, ACT>(a, p, sums, st);
     else if (p.tpr == 512) backward_rows<T, V, 512, 2 * K, ACT>(a, p, sums, st);
+    else if (p.tpr == 1024) backward_rows<T, V, 1024, 2 * K, ACT>(a, p, sums, st);
     else {
       a.chunks = p.chunks;
       const int64_t items = a.rows * a.chunks;
-      void* args[] = {&a};
+      int slices = p.few && !a.dx ? 0 : (int)p.groups;
+      void *one[] = {&a}, *two[] = {&a, &slices};
       if (a.dx)
         launch((const void*)layer_norm_chunk_backward_sums_kernel<T, V, ACT>, (unsigned)(items < 1 << 20 ? items : 1 << 20),
-               kThreads, args, st);
-      int slices = (int)p.groups;
-      void* more[] = {&a, &slices};
-      launch(sums ? (const void*)layer_norm_chunk_backward_kernel<T, V, ACT, true>
-                  : (const void*)layer_norm_chunk_backward_kernel<T, V, ACT, false>,
-             (unsigned)(p.groups * p.chunks), kThreads, more, st);
+               kThreads, one, st);
+      if (sums && p.few)
+        launch((const void*)layer_norm_chunk_backward_few_kernel<T, V, ACT>,
+               (unsigned)(slices * p.chunks + (a.cols + 4 * V - 1) / (4 * V)), kThreads, two, st);
+      else
+        launch(sums ? (const void*)layer_norm_chunk_backward_kernel<T, V, ACT, true>
+                    : (const void*)layer_norm_chunk_backward_kernel<T, V, ACT, false>,
+               (unsigned)(p.groups * p.chunks), kThreads, two, st);
     }
   }
-  if (sums) {
+  if (sums && !(p.few && a.rows > 0)) {
     int count = (int)p.groups;
     void* args[] = {&a, &count};
     const int64_t width = (a.cols + 3) / 4 * 4;
