@@ -280,8 +280,9 @@ int rbl_engine_stats(rbl_engine* e, rbl_kernel_stats* out, int reset);
 /* ---- training operators: what lies between the matrix products of Net2 (cfvpy/models.py:41-53) and between the backward pass
  * and the optimizer (cfvpy/selfplay.py:418-439).  All pointers named _dev are device memory of `device`; the work is enqueued on
  * `stream` (a hipStream_t of that device; NULL: its default stream) and nothing waits for it.  No state is kept from call to
- * call: what a call needs beside its operands is the workspace that the caller gives it, which no two calls in flight may
- * share.  Everything here may be captured into a HIP graph.  Results do not depend on timing: there are no atomics. ---- */
+ * call: what a call needs beside its operands is the workspace that the caller gives it (aligned to 16 bytes), which no two
+ * calls in flight may share.  Outputs must not overlap inputs, but for the gradients that are scaled in place.  Operands need
+ * the alignment of their elements, stats_dev that of 8 bytes.  Everything here may be captured into a HIP graph.  Results do not depend on timing: there are no atomics. ---- */
 enum { RBL_F32 = 0, RBL_F16 = 1, RBL_BF16 = 2 };
 enum { RBL_ACT_NONE = 0, RBL_ACT_GELU = 1 /* x/2 (1 + erf(x / sqrt 2)) */ };
 

@@ -256,6 +256,7 @@ void check(const rbl_grad* grads, int n) {
     if (grads[i].numel > 0 && !grads[i].data_dev) throw std::runtime_error("gradients: a tensor's data is null");
     if (grads[i].dtype != RBL_F32 && grads[i].dtype != RBL_F16 && grads[i].dtype != RBL_BF16)
       throw std::runtime_error("gradients: unknown dtype");
+    check_aligned(grads[i].data_dev, size_of(grads[i]), "gradients: a tensor's data");
   }
 }
 void check_norm(int norm) {
@@ -266,6 +267,7 @@ void check_workspace(const Plan& p, const void* workspace, int64_t bytes) {
   const int64_t need = workspace_size(p);
   if (bytes < need || (need > 0 && !workspace))
     throw std::runtime_error("gradients: the workspace must hold " + std::to_string(need) + " bytes");
+  check_aligned(workspace, 8, "gradients: the workspace");
 }
 void check_bound(double max_norm) {
   if (!(max_norm >= 0)) throw std::runtime_error("gradients: max_norm must be a number >= 0");

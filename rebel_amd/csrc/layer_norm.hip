@@ -1,4 +1,6 @@
 // rebel_amd/csrc/layer_norm.hip -- the C entries of layer normalisation: checks, workspaces, the choice of the element type.
+#include <initializer_list>
+
 #include "layer_norm.h"
 
 namespace rbl {
@@ -34,6 +36,14 @@ int64_t backward_workspace(const rbl_layer_norm_shape& s) {
 void check_workspace(int64_t need, const void* workspace, int64_t bytes) {
   if (bytes < need || (need > 0 && !workspace))
     throw std::runtime_error("layer norm: the workspace must hold " + std::to_string(need) + " bytes");
+}
+
+void check_pointers(const rbl_layer_norm_shape& s, const void* workspace, const void* stats, std::initializer_list<const void*> rows,
+                    std::initializer_list<const void*> params) {
+  check_aligned(workspace, 16, "layer norm: the workspace");
+  check_aligned(stats, 8, "layer norm: stats");
+  for (const void* p : rows) check_aligned(p, s.dtype == RBL_F32 ? 4 : 2, "layer norm: x, y, dy and dx");
+  for (const void* p : params) check_aligned(p, s.param_dtype == RBL_F32 ? 4 : 2, "layer norm: weight, bias and their gradients");
 }
 
 NormArgs args_of(const rbl_layer_norm_shape& s) {
@@ -76,6 +86,7 @@ int rbl_layer_norm_forward(int device, const rbl_layer_norm_shape* s, const void
     a.stats = stats_dev;
     a.partial = (float*)workspace_dev;
     rbl::check_workspace(rbl::forward_workspace(*s), workspace_dev, workspace_bytes);
+    rbl::check_pointers(*s, workspace_dev, stats_dev, {x_dev, y_dev}, {weight_dev, bias_dev});
     rbl::DeviceScope scope(device);
     const auto run = s->dtype == RBL_F32   ? rbl::layer_norm_forward<float>
                      : s->dtype == RBL_F16 ? rbl::layer_norm_forward<_Float16>
@@ -100,6 +111,7 @@ int rbl_layer_norm_backward(int device, const rbl_layer_norm_shape* s, const voi
     a.dw = dweight_dev;
     a.db = dbias_dev;
     rbl::check_workspace(rbl::backward_workspace(*s), workspace_dev, workspace_bytes);
+    rbl::check_pointers(*s, workspace_dev, stats_dev, {x_dev, dy_dev, dx_dev}, {weight_dev, bias_dev, dweight_dev, dbias_dev});
     const rbl::BackwardPlan p = rbl::backward_plan(*s);
     a.row_sums = (float*)workspace_dev;
     a.partial = a.row_sums + (rbl::backward_row_sums(*s, p) + 15) / 16 * 4;

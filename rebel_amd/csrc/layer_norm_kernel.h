@@ -632,37 +632,40 @@ __global__ __launch_bounds__(kSumsThreads) void layer_norm_sums_kernel(NormArgs 
   __shared__ float part[kSumsThreads / 64][COLS];
   const int width = (a.cols + 3) / 4 * 4;
   const int quad = threadIdx.x % LANES, slice = threadIdx.x / LANES;
-  const int64_t col = (int64_t)blockIdx.x * COLS + quad * 4;
   typedef Pack<float, 4>::type vec;
-  float s[4] = {0, 0, 0, 0};
-  if (col < 2 * (int64_t)width) {
+  for (int64_t first = (int64_t)blockIdx.x * COLS; first < 2 * (int64_t)width; first += (int64_t)gridDim.x * COLS) {
+    const int64_t col = first + quad * 4;
+    float s[4] = {0, 0, 0, 0};
+    if (col < 2 * (int64_t)width) {
 #pragma unroll 4
-    for (int g = slice; g < count; g += SLICES) {
-      const vec v = *(const vec*)(a.partial + (int64_t)g * 2 * width + col);
+      for (int g = slice; g < count; g += SLICES) {
+        const vec v = *(const vec*)(a.partial + (int64_t)g * 2 * width + col);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] += v[i];
+        for (int i = 0; i < 4; ++i) s[i] += v[i];
+      }
     }
-  }
 #pragma unroll
-  for (int d = LANES; d < 64; d *= 2)
+    for (int d = LANES; d < 64; d *= 2)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] += __shfl_xor(s[i], d);
-  if (threadIdx.x % 64 < LANES) {
+      for (int i = 0; i < 4; ++i) s[i] += __shfl_xor(s[i], d);
+    if (threadIdx.x % 64 < LANES) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part[threadIdx.x / 64][quad * 4 + i] = s[i];
-  }
-  lds_barrier();
-  const int64_t mine = (int64_t)blockIdx.x * COLS + threadIdx.x;
-  if (threadIdx.x < COLS && mine < 2 * (int64_t)width) {
-    float v = part[0][threadIdx.x];
-#pragma unroll
-    for (int k = 1; k < kSumsThreads / 64; ++k) v += part[k][threadIdx.x];
-    const bool second = mine >= width;
-    const int c = (int)(mine - (second ? width : 0));
-    if (c < a.cols) {
-      if (second && a.db) put_param<T>(a, a.db, c, v);
-      if (!second && a.dw) put_param<T>(a, a.dw, c, v);
+      for (int i = 0; i < 4; ++i) part[threadIdx.x / 64][quad * 4 + i] = s[i];
     }
+    lds_barrier();
+    const int64_t mine = first + threadIdx.x;
+    if (threadIdx.x < COLS && mine < 2 * (int64_t)width) {
+      float v = part[0][threadIdx.x];
+#pragma unroll
+      for (int k = 1; k < kSumsThreads / 64; ++k) v += part[k][threadIdx.x];
+      const bool second = mine >= width;
+      const int c = (int)(mine - (second ? width : 0));
+      if (c < a.cols) {
+        if (second && a.db) put_param<T>(a, a.db, c, v);
+        if (!second && a.dw) put_param<T>(a, a.dw, c, v);
+      }
+    }
+    lds_barrier();  // part is written again
   }
 }
 
@@ -903,7 +906,7 @@ void run_backward(NormArgs a, const BackwardPlan& p, hipStream_t st) {
     const int64_t width = (a.cols + 3) / 4 * 4;
     const bool few = 2 * width < 64 * kCus / 2;
     launch(few ? (const void*)layer_norm_sums_kernel<T, 16> : (const void*)layer_norm_sums_kernel<T, 64>,
-           (unsigned)((2 * width + (few ? 15 : 63)) / (few ? 16 : 64)), kSumsThreads, args, st);
+           (unsigned)std::min((2 * width + (few ? 15 : 63)) / (few ? 16 : 64), (int64_t)1 << 20), kSumsThreads, args, st);
   }
 }
 

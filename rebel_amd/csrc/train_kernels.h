@@ -29,6 +29,10 @@ int train_entry(F&& f) {
   return 1;
 }
 
+inline void check_aligned(const void* p, uintptr_t bytes, const char* what) {
+  if ((uintptr_t)p % bytes) throw std::runtime_error(std::string(what) + " must be aligned to " + std::to_string(bytes) + " bytes");
+}
+
 // Selects the device for the launches of one call; the one that was current is current again afterwards.  Made after the
 // arguments have been checked, so that a refusal needs no GPU.
 class DeviceScope {

@@ -58,7 +58,12 @@ int64_t row_stride(const Tensor& t) {
   return step < 0 ? sizes[d] : step;
 }
 
-Tensor with_rows(const Tensor& t) { return row_stride(t) < 0 ? t.contiguous() : t; }
+// What the kernels can read: values as they lie in memory (a view may be marked as negated), rows at one distance.
+Tensor with_rows(const Tensor& t) {
+  const Tensor v = t.is_neg() ? t.resolve_neg() : t;
+  return row_stride(v) < 0 ? v.contiguous() : v;
+}
+Tensor dense(const Tensor& t) { return !t.defined() ? t : t.is_neg() ? t.resolve_neg().contiguous() : t.contiguous(); }
 
 Tensor workspace(const Tensor& like, int64_t bytes) {
   check(bytes < 0);
@@ -178,7 +183,7 @@ Tensor layer_norm(const Tensor& x_in, const OptTensor& weight, const OptTensor& 
   check_arguments(x_in, w_in, b_in);
   // what is copied for its layout is copied where its gradient does not see it: the edges lead to the arguments themselves
   std::optional<at::AutoDispatchBelowADInplaceOrView> plain(std::in_place);
-  const Tensor x = with_rows(x_in), w = w_in.defined() ? w_in.contiguous() : w_in, b = b_in.defined() ? b_in.contiguous() : b_in;
+  const Tensor x = with_rows(x_in), w = dense(w_in), b = dense(b_in);
   const bool grad = at::GradMode::is_enabled() && (x_in.requires_grad() || (w_in.defined() && w_in.requires_grad()) ||
                                                    (b_in.defined() && b_in.requires_grad()));
   if (!grad) return forward(x, w, b, eps, activation, nullptr);
@@ -239,6 +244,8 @@ Gradients gather(const std::vector<const Tensor*>& tensors, bool scaled) {
       spans.push_back({at, at + t.numel() * t.element_size()});
     }
     g.list.push_back({at_data, t.numel(), type});
+    // as every operation in place: who has saved the tensor for a gradient finds out
+    if (scaled && !t.is_inference()) torch::autograd::impl::bump_version(t);
   }
   std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
   for (size_t i = 1; i < spans.size(); ++i)

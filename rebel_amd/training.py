@@ -30,13 +30,15 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, activation=None):
     """
     if activation not in ACTIVATIONS:
         raise ValueError(f"layer_norm: activation must be None or 'gelu', not {activation!r}")
+    if torch.jit.is_tracing():
+        raise ValueError("layer_norm: a trace would keep its result as a constant; trace the LayerNorm module")
     return _train.layer_norm(x, weight, bias, eps, ACTIVATIONS[activation])
 
 
 class LayerNorm(nn.Module):
     """nn.LayerNorm over the last dimension (same parameters, same state_dict) on layer_norm; `activation` as there.
 
-    A scripted copy holds torch's own operators, so that a saved TorchScript file needs nothing of this package.
+    A scripted or traced copy holds torch's own operators, so that a saved TorchScript file needs nothing of this package.
     """
 
     def __init__(self, normalized_shape, eps=1e-5, elementwise_affine=True, bias=True, activation=None, device=None, dtype=None):
@@ -57,7 +59,7 @@ class LayerNorm(nn.Module):
             self.register_parameter("bias", None)
 
     def forward(self, x):
-        if torch.jit.is_scripting():
+        if torch.jit.is_scripting() or torch.jit.is_tracing():
             y = nn.functional.layer_norm(x, self.normalized_shape, self.weight, self.bias, self.eps)
             return y if self.activation is None else nn.functional.gelu(y)
         else:
@@ -73,7 +75,7 @@ def grad_norm(tensors, norm_type=2.0):
 
     Sums are held in 64 bits.  float32, float16 and bfloat16 tensors may be mixed; all must be on one GPU.
     """
-    return _train.grad_norm(_as_list(tensors), norm_type)
+    return _train.grad_norm(_as_list(tensors), float(norm_type))
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
@@ -83,7 +85,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     that is not finite scales all the same unless error_if_nonfinite (which waits for the norm on the host).  Gradients that
     share memory are refused.
     """
-    return _train.clip_grad_norm(_as_list(parameters), max_norm, norm_type, error_if_nonfinite)
+    return _train.clip_grad_norm(_as_list(parameters), float(max_norm), float(norm_type), error_if_nonfinite)
 
 
 def _as_list(tensors):

@@ -174,6 +174,97 @@ def test_layer_norm_strides(dtype):
 
 
 @gpu
+def test_layer_norm_of_other_views():
+    """Windows that overlap in memory, and views that torch marks as negated without touching the memory."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    line = torch.randn(400, generator=g, device="cuda")
+    w, b = (torch.randn(300, generator=g, device="cuda") for _ in range(2))
+    windows = line.unfold(0, 300, 7)
+    dy = torch.randn(windows.shape, generator=g, device="cuda")
+    want = oracle(windows, w, b, dy, True)
+    for name, got in zip(("y", "dx", "dw", "db"), run(windows, w, b, dy, "gelu")):
+        near(got, want[name], name)
+    x = torch.randn(15, 300, generator=g, device="cuda")
+    want = oracle(-x, -w, -b, -dy, True)
+    neg = torch._neg_view
+    for name, got in zip(("y", "dx", "dw", "db"), run(neg(x), neg(w), neg(b), neg(dy), "gelu")):
+        near(got, want[name], name)
+    p = torch.nn.Parameter(torch.empty_like(x))
+    p.grad = neg(x.clone())
+    training.clip_grad_norm_([p], 1.0)
+    v = -x.double() / (float(clip_oracle([x], 2)) + 1e-6)
+    near(p.grad, (v, v.abs() * 3 * U))
+
+
+@gpu
+def test_layer_norm_guards_what_it_has_saved():
+    x, w, b, dy = make(5, 64, torch.float32, torch.float32)
+    for act, touched, fails in ((None, 0, True), ("gelu", 1, True), ("gelu", 2, True), (None, 2, False)):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        y = training.layer_norm(*leaves, activation=act)
+        with torch.no_grad():
+            leaves[touched].mul_(2)
+        if fails:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(y, leaves, dy)
+        else:  # the bias is not needed without an activation
+            torch.autograd.grad(y, leaves, dy)
+    y = training.layer_norm(*leaves)
+    torch.autograd.grad(y, leaves, dy)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, leaves, dy)
+    p = torch.nn.Parameter(torch.zeros(4, device="cuda"))
+    p.grad = torch.ones(4, device="cuda")
+    before = p.grad._version
+    training.clip_grad_norm_([p], 1.0)
+    assert p.grad._version == before + 1
+
+
+@gpu
+def test_operators_from_several_threads():
+    from concurrent.futures import ThreadPoolExecutor
+
+    x, w, b, dy = make(300, 700, torch.float32, torch.float32)
+    want = run(x, w, b, dy, "gelu")
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            out = []
+            for _ in range(10):
+                (p,) = holders([x.clone()])
+                out.append((run(x, w, b, dy, "gelu"), training.clip_grad_norm_([p], 1.0, error_if_nonfinite=k % 2 == 0), p.grad))
+            torch.cuda.current_stream().synchronize()
+            return out
+
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(4) as pool:
+        results = [r for rs in pool.map(work, range(4)) for r in rs]
+    for got, norm, grad in results:
+        assert all(torch.equal(p, q) for p, q in zip(got, want)) and torch.equal(norm, results[0][1])
+        assert (grad - results[0][2]).abs().max() <= 4 * U * grad.abs().max()  # the factor from the norm in f64 or in f32
+
+
+@gpu
+def test_layer_norm_of_one_row_of_many_columns():
+    """More columns than one launch has work-items for at 16 columns to a workgroup of the join."""
+    n = 2 ** 27 + 5
+    x = torch.randn(2, n, device="cuda")
+    dy = torch.randn(2, n, device="cuda")
+    w = torch.ones(n, device="cuda")
+    y, dx, dw, db = run(x, w, torch.zeros_like(w), dy, None)
+    assert torch.equal(db, dy[0] + dy[1])
+    mean = torch.stack([r.double().mean() for r in x])
+    inv = torch.stack([(r.double().var(unbiased=False) + EPS).rsqrt() for r in x])
+    depth = n / 4096 + 64  # a chunk's chain is short, the join's has the chunks of a lane
+    for cols in (slice(0, 1000), slice(2 ** 26, 2 ** 26 + 1000), slice(n - 1000, n)):
+        h = (x[:, cols].double() - mean[:, None]) * inv[:, None]
+        eh = (h.abs() + 1) * (depth + 8) * U
+        near(y[:, cols], (h, eh))
+        terms = h * dy[:, cols].double()
+        near(dw[cols], (terms.sum(0), (eh * dy[:, cols].double().abs()).sum(0) + 4 * U * terms.abs().sum(0)))
+
+
+@gpu
 @pytest.mark.parametrize("cols", [5, 256, 1000, 20000, 70000])
 def test_layer_norm_of_no_rows(cols):
     w = torch.ones(cols, device="cuda", requires_grad=True)
@@ -408,7 +499,13 @@ def test_capture_with_a_live_eager_graph_is_refused():
             out["said"] = str(ex)
         with torch.no_grad():
             out["y"] = training.layer_norm(x, w, b)
-    assert "outside this capture" in out["said"]
+        p = torch.nn.Parameter(torch.zeros(4, device="cuda"))
+        p.grad = torch.zeros(4, device="cuda")
+        try:
+            training.clip_grad_norm_([p], 1.0, error_if_nonfinite=True)
+        except ValueError as ex:
+            out["clip"] = str(ex)
+    assert "outside this capture" in out["said"] and "a capture cannot do" in out["clip"]
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out["y"], alive)
@@ -590,7 +687,7 @@ def test_a_training_step_of_the_value_net(batch, bound):
     # the trained net goes on as any other: the scripted form and the plain class hold the same values
     plain = Net2(num_faces=6, num_dice=1, n_hidden=256, use_layer_norm=True, n_layers=2).cuda()
     plain.load_state_dict(net.state_dict())
-    for other in (plain, torch.jit.script(net)):
+    for other in (plain, torch.jit.script(net), torch.jit.trace(net, q[:1])):
         assert (net(q) - other(q)).abs().max() <= 1e-4
 
 
@@ -633,6 +730,8 @@ def test_layer_norm_refuses():
             training.LayerNorm(size)
     with pytest.raises(ValueError, match="no CPU path"):
         training.LayerNorm(8)(x)
+    with pytest.raises(ValueError, match="constant"):
+        torch.jit.trace(training.layer_norm, x)
     with pytest.raises(ValueError, match="use_layer_norm"):
         Net2(num_faces=4, num_dice=1, native=True)
 
@@ -694,6 +793,12 @@ def test_c_entries_refuse():
                 said(call(s, space=one, n=need - 1), "workspace")
                 said(call(s, space=None, n=need), "workspace")
 
+    s = shape(4, 20_000)  # one that needs no workspace forward and one backward
+    for call, word in ((lambda: fwd(s, x=C.c_void_p(18)), "x, y, dy and dx"), (lambda: fwd(s, y=C.c_void_p(17)), "x, y, dy and dx"),
+                       (lambda: bwd(s, dy=C.c_void_p(18)), "x, y, dy and dx"), (lambda: bwd(s, stats=C.c_void_p(20)), "stats"),
+                       (lambda: bwd(s, space=C.c_void_p(24)), "workspace must be aligned")):
+        said(call(), word)
+
     def clip(grads, n=None, norm=capi.NORM_2, bound=1.0, out=one, space=one, size=1 << 40, which=L.rbl_grad_clip):
         a = (capi.Grad * max(1, len(grads)))(*[capi.Grad(*g) for g in grads])
         n = len(grads) if n is None else n
@@ -714,6 +819,8 @@ def test_c_entries_refuse():
         said(clip([(16, 4, 0)], norm=4, which=which), "norm must be")
         said(clip([(16, 4, 0)], size=7, which=which), "workspace")
         said(clip([(16, 4, 0)], space=None, which=which), "workspace")
+        said(clip([(16, 4, 0)], space=C.c_void_p(20), which=which), "aligned")
+        said(clip([(18, 4, 0)], which=which), "aligned")
     for which in (L.rbl_grad_clip, L.rbl_grad_scale):
         said(clip([(16, 4, 0)], bound=-1.0, which=which), "max_norm")
         said(clip([(16, 4, 0)], bound=math.nan, which=which), "max_norm")
