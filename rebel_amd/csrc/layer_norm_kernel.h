@@ -8,6 +8,11 @@
 //
 // h is computed again from x and the two statistics of the row, so nothing else is kept between the passes.
 //
+// All of it is bound by memory where the tensors are large: 8 to 15 instructions an element, 20 more for the GELU, whose
+// exponential and reciprocal count fourfold.  (f32 + GELU hides behind the memory; 16-bit rows + GELU do not: 8192 x 12000 bf16
+// takes 134 us with it and 87 without.)  So a row is read once and stays in registers, and a thread has as many of its elements
+// as fit there: what is done once per row and thread (two sums over the group, the statistics) is then done least often.
+//
 // The element types are compiled apart (layer_norm_f32.hip, layer_norm_f16.hip, layer_norm_bf16.hip); layer_norm.hip holds the C
 // entries.
 #pragma once
@@ -20,8 +25,8 @@ namespace {
 
 // Phi(z) and exp(-z^2 / 2).  For x = |z|: Phi(-x) = exp(-x^2 / 2) P(x) with P(x) = exp(x^2 / 2) erfc(x / sqrt 2) / 2, which
 // falls smoothly from 1/2 like 1 / (x sqrt(2 pi)): a polynomial of degree 8 in u = 1 / (1 + 0.3 x) without a constant term
-// (the form of Abramowitz and Stegun 7.1.26; coefficients fitted here to the least relative error on [0, 14], 1.5e-7 exactly
-// and 4.3e-7 in f32).  The error is RELATIVE on the negative side too, where 1 + erf would cancel, and the exponential is
+// (the form of Abramowitz and Stegun 7.1.26; coefficients from scripts/fit_normal_cdf.py, least relative error on [0, 14]:
+// 1.5e-7 exactly, 4.3e-7 in f32).  The error is RELATIVE on the negative side too, where 1 + erf would cancel, and the exponential is
 // the one that the derivative needs.  NaN stays NaN; +-inf give 1 and 0.
 __device__ __forceinline__ float normal_cdf(float z, float* density_exp) {
   const float x = __builtin_fabsf(z);
@@ -199,7 +204,10 @@ __device__ __forceinline__ void statistics(const float (&x)[K][V], const Place<V
 template <int TPR>
 constexpr int forward_threads() { return TPR <= 64 ? 256 : TPR; }
 
-// Forward, a row in the registers of TPR threads (K vectors of V elements each): read once, written once.
+// Forward, a row in the registers of TPR threads (K vectors of V elements each): read once, written once.  As many workgroups as
+// the chip holds, each with the same number of rows, the parameters in registers and the next row on its way.  Bound by memory:
+// 270336 x 256 f32 + GELU 103 us (5.4 TB/s; with 4 elements to a thread instead of 16 it was 149), 8192 x 4096 bf16 23.4 us (5.7),
+// 32768 x 8192 bf16 178 us (6.0).  One row of 256: 2.2 us, a load, two sums and a store one after the other.
 template <class T, int V, int TPR, int K, bool EVEN, int ACT, bool STREAM>
 __global__ __launch_bounds__(forward_threads<TPR>()) void layer_norm_forward_kernel(NormArgs a) {
   constexpr int NT = forward_threads<TPR>(), RPB = NT / TPR;
@@ -255,8 +263,10 @@ __global__ __launch_bounds__(forward_threads<TPR>()) void layer_norm_forward_ker
   }
 }
 
-// Rows that are longer than a workgroup's registers: chunks of kChunk vectors, each with its own mean and sum of squared
-// deviations, which the second kernel joins (Chan's formula) before it normalises its chunk.
+// Rows that are longer than a workgroup's registers: chunks of kChunkK vectors to a thread, each with its own mean and sum of
+// squared deviations, which the second kernel joins (Chan's formula) before it normalises its chunk.  x is read twice: 2000 x 65537
+// f32 306 us (5.1 TB/s of three passes), 24 x 65537 3.8 + 5.6 us.  Batches of rows small enough for the second reading to come
+// from the 256 MB cache were not faster (4096 x 65537: 608 us in one, 626 in batches of 128 MB).
 template <int V>
 constexpr int chunk_cols() { return kThreads * kChunkK * V; }
 
@@ -366,7 +376,8 @@ __device__ __forceinline__ void put_sums(float* out, const float (&v)[V], int sk
 
 // Backward, a row in the registers of TPR threads: x and dy are read once, dx is written, and (SUMS) g h and g are summed up over
 // the rows of the workgroup, in registers (rows of 1024 threads: in LDS, each thread its own 16-byte cells); the workgroups' sums
-// are joined by layer_norm_sums_kernel.  Workgroup `group` of `groups`.
+// are joined by layer_norm_sums_kernel.  Bound by memory: 270336 x 256 f32 + GELU 150 us (5.5 TB/s), 32768 x 8192 bf16 265 us (6.1),
+// 8192 x 16384 bf16 173 us (4.7).  Workgroup `group` of `groups`.
 template <class T, int V, int TPR, int K, bool EVEN, int ACT, bool SUMS, bool STREAM>
 __device__ __forceinline__ void backward_of_rows(const NormArgs& a, int group, int groups) {
   constexpr int NT = backward_threads(TPR), RPB = NT / TPR;
@@ -704,7 +715,8 @@ __global__ __launch_bounds__(kThreads) void layer_norm_chunk_backward_sums_kerne
   }
 }
 
-// ... then dx, and the parameters' gradients summed up over every `slices`-th row of a chunk
+// ... then dx, and the parameters' gradients summed up over every `slices`-th row of a chunk.  x and dy are read twice: 2000 x 65537
+// f32 562 us for both kernels (4.7 TB/s of five passes).
 template <class T, int V, int ACT, bool SUMS>
 __device__ __forceinline__ void backward_of_chunk(const NormArgs& a, int block, int slices) {
   typedef typename Pack<T, V>::type vec;
@@ -816,14 +828,13 @@ void forward_rows(const NormArgs& a, hipStream_t st) {
   even ? forward_launch<T, V, TPR, K, true, ACT, false>(a, st) : forward_launch<T, V, TPR, K, false, ACT, false>(a, st);
 }
 
-
 template <class T, int ACT>
 void run_forward(NormArgs a, hipStream_t st) {
   constexpr int V = 16 / sizeof(T);
   if (a.rows == 0) return;
   // 16 elements to a thread: fewer leave too much of the work on a row's two sums, more spill out of the registers
   constexpr int K = 16 / V;
-  if (a.cols < V) return forward_rows<T, 1, 4, 2, ACT>(a, st);
+  if (a.cols < V) return forward_launch<T, 1, 4, 2, false, ACT, false>(a, st);
   if (a.cols <= 64) return forward_rows<T, V, 4, K, ACT>(a, st);
   if (a.cols <= 128) return forward_rows<T, V, 8, K, ACT>(a, st);
   if (a.cols <= 256) return forward_rows<T, V, 16, K, ACT>(a, st);
@@ -844,18 +855,18 @@ void run_forward(NormArgs a, hipStream_t st) {
 
 template <class T, int V, int TPR, int K, int ACT>
 void backward_rows(NormArgs a, const BackwardPlan& p, bool sums, hipStream_t st) {
-  const bool even = a.cols == TPR * K * V;
+  const bool even = V > 1 && a.cols == TPR * K * V;  // V = 1: rows of fewer elements than a vector has
   if (sums && p.few) {
     int row_groups = a.dx ? (int)p.groups : 0;
     void* args[] = {&a, &row_groups};
-    launch(even ? (const void*)layer_norm_backward_few_kernel<T, V, TPR, K, true, ACT>
+    launch(even ? (const void*)layer_norm_backward_few_kernel<T, V, TPR, K, (V > 1), ACT>
                 : (const void*)layer_norm_backward_few_kernel<T, V, TPR, K, false, ACT>,
            (unsigned)(row_groups + (a.cols + 4 * V - 1) / (4 * V)), backward_threads(TPR), args, st);
     return;
   }
-  const void* kernel = sums ? even ? (const void*)layer_norm_backward_kernel<T, V, TPR, K, true, ACT, true, false>
+  const void* kernel = sums ? even ? (const void*)layer_norm_backward_kernel<T, V, TPR, K, (V > 1), ACT, true, false>
                                    : (const void*)layer_norm_backward_kernel<T, V, TPR, K, false, ACT, true, false>
-                       : even ? (const void*)layer_norm_backward_kernel<T, V, TPR, K, true, ACT, false, false>
+                       : even ? (const void*)layer_norm_backward_kernel<T, V, TPR, K, (V > 1), ACT, false, false>
                               : (const void*)layer_norm_backward_kernel<T, V, TPR, K, false, ACT, false, false>;
   if constexpr (TPR >= 16) {
     if (sums && beyond_caches<T>(a))
