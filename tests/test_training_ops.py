@@ -540,6 +540,9 @@ CLIP_SETS = {
     "one value": [(1, "f32")], "one odd": [(4097, "bf16")], "small": [(n, "f32") for n in (6912, 256, 256, 256, 65536, 256, 256, 256, 1536, 6)],
     "types": [(1000, "f32"), (1001, "f16"), (999, "bf16"), (0, "f32"), (3, "f16"), (250_001, "f32")],
     "many": [(1 + 37 * i % 5000, ("f32", "bf16", "f16")[i % 3]) for i in range(700)], "large": [(9_000_001, "f32"), (7_000_003, "bf16")],
+    "tiny": [(1, "bf16"), (3, "f16"), (2, "f32"), (7, "bf16"), (9, "f16"), (2048, "bf16"), (2049, "bf16"), (1024, "f32"), (1027, "f32"), (8, "f16")],
+    "pairs": [(1024, "f32"), (2048, "f16")] * 48, "one more": [(1024, "f32"), (2048, "bf16")] * 48 + [(1, "f32")],
+    "384 KB": [(98304, "f32")], "384 KB and one": [(98305, "f32")],
     "scattered": [(0, "f32")] * 140 + [(5, "f32")] + [(0, "bf16")] * 3 + [(70, "bf16")] * 129}
 
 
