@@ -7,10 +7,10 @@
 // the two has added them up).  Squares are formed and summed in f64: no
 // gradient that is finite in f32 overflows or vanishes on the way, and the order of the sum does not show in an f32 result.
 // Bound by memory, one reading for the sums and one reading and one writing for the scaling: 400 M f32 in 200 tensors 238 us (6.7 TB/s)
-// and 637 us (5.0 TB/s).  A step whose norm stays under the bound ends after the sums.  Small sets are bound by the two launches:
-// 3.8 us each for the 76 thousand values of a net of two hidden layers of 256, the latency of one load after the other (finding the
-// tensor by all lanes at once, or loading a short chunk in one batch, made them no shorter and the large ones longer; one workgroup
-// that keeps such a set in its registers took 10.5 us, most of it for its 300 KB through one CU).
+// and 637 us (5.0 TB/s).  A step whose norm stays under the bound ends after the sums.  Small sets are bound by
+// latency, one load after the other: 3.0 and 3.6 us for the 76 thousand values of a net of two hidden layers of 256, with the chunks
+// themselves in the arguments (3.8 and 4.0 with a search for the tensor).  One workgroup that keeps such a set in its registers took
+// 10.5 us, most of it for its 300 KB through one CU.
 //
 // The table of tensors travels in the kernel's arguments, as many as fit in 4 KB to a launch: nothing is copied to the device
 // beforehand, so a captured call replays with the pointers it was captured with and needs no memory of the host's.
@@ -36,6 +36,13 @@ struct GradTable {
 };
 constexpr int kTypeShift = 30;
 
+// Sets of few chunks: the chunks themselves, found without a search.
+constexpr int kFewChunks = 320;
+struct ChunkTable {
+  void* data[kFewChunks];
+  unsigned count[kFewChunks];  // elements; their type in the upper two bits
+};
+
 struct ClipArgs {
   double* sums;          // one per chunk, then their sum
   const float* norm_in;  // the norm, where it is known already
@@ -46,7 +53,7 @@ struct ClipArgs {
   int first;  // chunks before the table's first
   int total;  // chunks of all tables
 };
-static_assert(sizeof(GradTable) + sizeof(ClipArgs) <= 4096, "kernel arguments");
+static_assert(sizeof(GradTable) + sizeof(ClipArgs) <= 4096 && sizeof(ChunkTable) + sizeof(ClipArgs) <= 4096, "kernel arguments");
 
 // One element's share of the norm, and how shares are joined: the sum, or the maximum that keeps a NaN.
 template <int NORM>
@@ -94,6 +101,10 @@ __device__ __forceinline__ Chunk chunk_of(const GradTable& t, const ClipArgs& a,
   return {t.data[lo], (int64_t)(index - t.first_chunk[lo]) * whole, is_last ? (int)(last & ((1u << kTypeShift) - 1)) : whole, type};
 }
 
+__device__ __forceinline__ Chunk chunk_of(const ChunkTable& t, const ClipArgs&, int index) {
+  return {t.data[index], 0, (int)(t.count[index] & ((1u << kTypeShift) - 1)), (int)(t.count[index] >> kTypeShift)};
+}
+
 // 16 bytes in one access, at the alignment of an element
 template <class T>
 struct Pack {
@@ -130,8 +141,8 @@ __device__ __forceinline__ double sum_chunk(const T* g, int count) {
   return join<NORM>(s[0], s[1]);
 }
 
-template <int NORM>
-__global__ __launch_bounds__(kThreads) void grad_sums_kernel(GradTable t, ClipArgs a) {
+template <int NORM, class TABLE>
+__global__ __launch_bounds__(kThreads) void grad_sums_kernel(TABLE t, ClipArgs a) {
   __shared__ double slots[kThreads / 64];
   const Chunk k = chunk_of(t, a, blockIdx.x);
   double v = k.type == RBL_F32   ? sum_chunk<float, NORM>((const float*)k.data + k.begin, k.count)
@@ -178,8 +189,8 @@ __device__ __forceinline__ void scale_chunk(T* g, int count, float c) {
 }
 
 // NORM 0: the norm is there already
-template <int NORM>
-__global__ __launch_bounds__(kThreads) void grad_scale_kernel(GradTable t, ClipArgs a) {
+template <int NORM, class TABLE>
+__global__ __launch_bounds__(kThreads) void grad_scale_kernel(TABLE t, ClipArgs a) {
   __shared__ double slots[kThreads / 64];
   double norm;
   if constexpr (NORM == 0) {
@@ -216,20 +227,18 @@ __global__ __launch_bounds__(kNormThreads) void grad_norm_kernel(ClipArgs a) {
   }
 }
 
-template <int NORM>
+// The kernels of a norm (0: it is known), for many chunks and for few
 struct Kernels {
-  static const void* sums() { return (const void*)grad_sums_kernel<NORM>; }
-  static const void* scale() { return (const void*)grad_scale_kernel<NORM>; }
-  static const void* norm() { return (const void*)grad_norm_kernel<NORM>; }
+  const void *sums, *sums_few, *scale, *scale_few, *norm;
 };
-const void* sums_kernel(int norm) {
-  return norm == RBL_NORM_1 ? Kernels<RBL_NORM_1>::sums() : norm == RBL_NORM_2 ? Kernels<RBL_NORM_2>::sums() : Kernels<RBL_NORM_INF>::sums();
+template <int NORM>
+Kernels kernels() {
+  return {(const void*)grad_sums_kernel<NORM, GradTable>, (const void*)grad_sums_kernel<NORM, ChunkTable>,
+          (const void*)grad_scale_kernel<NORM, GradTable>, (const void*)grad_scale_kernel<NORM, ChunkTable>,
+          (const void*)grad_norm_kernel<NORM>};
 }
-const void* scale_kernel(int norm) {
-  return norm == RBL_NORM_1 ? Kernels<RBL_NORM_1>::scale() : norm == RBL_NORM_2 ? Kernels<RBL_NORM_2>::scale() : Kernels<RBL_NORM_INF>::scale();
-}
-const void* norm_kernel(int norm) {
-  return norm == RBL_NORM_1 ? Kernels<RBL_NORM_1>::norm() : norm == RBL_NORM_2 ? Kernels<RBL_NORM_2>::norm() : Kernels<RBL_NORM_INF>::norm();
+Kernels kernels_of(int norm) {
+  return norm == RBL_NORM_1 ? kernels<RBL_NORM_1>() : norm == RBL_NORM_2 ? kernels<RBL_NORM_2>() : kernels<RBL_NORM_INF>();
 }
 
 int64_t size_of(const rbl_grad& g) { return g.dtype == RBL_F32 ? 4 : 2; }
@@ -279,10 +288,28 @@ void check_bound(double max_norm) {
   if (!(max_norm >= 0)) throw std::runtime_error("gradients: max_norm must be a number >= 0");
 }
 
-// One launch of `kernel` for every table of tensors; `backwards`: the last table first
-void for_tables(const void* kernel, const rbl_grad* grads, int n, ClipArgs a, const Plan& p, bool backwards, hipStream_t st) {
+// One launch of `kernel` for every table of tensors, or of `few` for all of few chunks; `backwards`: the last table first
+void for_tables(const void* kernel, const void* few, const rbl_grad* grads, int n, ClipArgs a, const Plan& p, bool backwards,
+                hipStream_t st) {
   a.chunk = 1 << p.shift;
   a.total = p.total;
+  if (p.total == 0) return;
+  if (p.total <= kFewChunks) {
+    ChunkTable c;
+    int count = 0;
+    for (int i = 0; i < n; ++i) {
+      const int64_t bytes = grads[i].numel * size_of(grads[i]);
+      for (int64_t at = 0; at < bytes; at += a.chunk) {
+        c.data[count] = (char*)grads[i].data_dev + at;
+        c.count[count++] = (unsigned)(std::min(bytes - at, (int64_t)a.chunk) / size_of(grads[i])) | (unsigned)grads[i].dtype << kTypeShift;
+      }
+    }
+    a.count = count;
+    a.first = 0;
+    void* args[] = {&c, &a};
+    launch(few, (unsigned)count, kThreads, args, st);
+    return;
+  }
   GradTable t;
   int from = 0, to = n, first = backwards ? a.total : 0;
   while (from < to) {
@@ -340,13 +367,14 @@ int rbl_grad_norm(int device, const rbl_grad* grads, int n, int norm, float* nor
     rbl::check_workspace(p, workspace_dev, workspace_bytes);
     if (!norm_dev) throw std::runtime_error("gradients: norm_dev is null");
     rbl::DeviceScope scope(device);
+    const rbl::Kernels k = rbl::kernels_of(norm);
     rbl::ClipArgs a{};
     a.sums = (double*)workspace_dev;
     a.norm_out = norm_dev;
-    rbl::for_tables(rbl::sums_kernel(norm), grads, n, a, p, false, (hipStream_t)stream);
+    rbl::for_tables(k.sums, k.sums_few, grads, n, a, p, false, (hipStream_t)stream);
     a.total = p.total;
     void* args[] = {&a};
-    rbl::launch(rbl::norm_kernel(norm), 1, rbl::kNormThreads, args, (hipStream_t)stream);
+    rbl::launch(k.norm, 1, rbl::kNormThreads, args, (hipStream_t)stream);
   });
 }
 
@@ -360,17 +388,18 @@ int rbl_grad_clip(int device, const rbl_grad* grads, int n, int norm, double max
     rbl::check_workspace(p, workspace_dev, workspace_bytes);
     if (!norm_dev) throw std::runtime_error("gradients: norm_dev is null");
     rbl::DeviceScope scope(device);
+    const rbl::Kernels k = rbl::kernels_of(norm);
     rbl::ClipArgs a{};
     a.sums = (double*)workspace_dev;
     a.norm_out = norm_dev;
     a.max_norm = max_norm;
-    rbl::for_tables(rbl::sums_kernel(norm), grads, n, a, p, false, (hipStream_t)stream);
+    rbl::for_tables(k.sums, k.sums_few, grads, n, a, p, false, (hipStream_t)stream);
     a.total = p.total;
     if (a.total == 0 || a.total > rbl::kSumsMost) {  // nothing to scale: the norm of nothing
       void* args[] = {&a};
-      rbl::launch(rbl::norm_kernel(norm), 1, rbl::kNormThreads, args, (hipStream_t)stream);
+      rbl::launch(k.norm, 1, rbl::kNormThreads, args, (hipStream_t)stream);
     }
-    rbl::for_tables(rbl::scale_kernel(norm), grads, n, a, p, true, (hipStream_t)stream);
+    rbl::for_tables(k.scale, k.scale_few, grads, n, a, p, true, (hipStream_t)stream);
   });
 }
 
@@ -383,7 +412,7 @@ int rbl_grad_scale(int device, const rbl_grad* grads, int n, double max_norm, co
     rbl::ClipArgs a{};
     a.norm_in = norm_dev;
     a.max_norm = max_norm;
-    rbl::for_tables((const void*)rbl::grad_scale_kernel<0>, grads, n, a, rbl::plan_of(grads, n), true, (hipStream_t)stream);
+    rbl::for_tables((const void*)rbl::grad_scale_kernel<0, rbl::GradTable>, (const void*)rbl::grad_scale_kernel<0, rbl::ChunkTable>, grads, n, a, rbl::plan_of(grads, n), true, (hipStream_t)stream);
   });
 }
 
