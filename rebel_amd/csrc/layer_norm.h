@@ -1,6 +1,8 @@
 // rebel_amd/csrc/layer_norm.h -- layer normalisation, host side: what the entries (layer_norm.hip) and the kernels' launchers
 // (layer_norm_kernel.h, compiled once for each element type) share.
 #pragma once
+#include <algorithm>
+
 #include "train_kernels.h"
 
 namespace rbl {
@@ -65,7 +67,12 @@ inline BackwardPlan backward_plan(const rbl_layer_norm_shape& s) {
     if (s.cols > 8192) p.tpr = 1024;
     const int nt = backward_threads(p.tpr);
     const int64_t need = (s.rows * p.tpr + nt - 1) / nt;
-    p.groups = p.few || need == 0 ? need : even_grid(need, (int64_t)kCus * (nt > kBackwardWaves * 64 ? 1 : kBackwardWaves * 64 / nt));
+    // Threads past the row's end have nothing to load.  16-bit rows have one vector to a thread, and make up for them with more
+    // workgroups (65536 x 1280 bf16 113 us instead of 131, 32768 x 2560 106 instead of 126); f32 rows have two, and are slower for it.
+    const int64_t threads = kBackwardWaves * 64;
+    int64_t per_cu = threads / nt;
+    if (s.dtype != RBL_F32 && s.cols <= 4096) per_cu = (threads * p.tpr * 8 + nt * s.cols / 2) / (nt * s.cols);
+    p.groups = p.few || need == 0 ? need : even_grid(need, kCus * std::clamp<int64_t>(per_cu, 1, 16));
   } else {
     p.chunks = chunks_of_row(s.cols, s.dtype == RBL_F32 ? 4 : 8);
     const int64_t most = (2 * kCus + p.chunks - 1) / p.chunks;  // eight wavefronts to a CU here too

@@ -84,12 +84,14 @@ struct Pack {
 template <int V, int TPR, int K, bool EVEN>
 struct Place {
   int col, skip;
+  bool busy;  // some lane of the wavefront owns something: the others leave its arithmetic out
   static __device__ __forceinline__ constexpr bool whole(int k) { return EVEN || (TPR >= 8 && 2 * k + 2 <= K); }
   Place() = default;
   __device__ __forceinline__ Place(int t, int k, int cols) {
     const int at = (t + k * TPR) * V;
     col = whole(k) || at + V <= cols ? at : cols - V;
     skip = whole(k) ? 0 : at - col;
+    busy = whole(k) || __builtin_amdgcn_readfirstlane(at) < cols;
   }
   __device__ __forceinline__ bool owns(int k, int i) const { return whole(k) || i >= skip; }
 };
@@ -249,6 +251,7 @@ __global__ __launch_bounds__(forward_threads<TPR>()) void layer_norm_forward_ker
     T* y = (T*)a.y + row * a.cols;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
+      if (!at[k].busy) continue;
       if (!KEEP) {
         __builtin_amdgcn_sched_barrier(0);  // not all of the parameters at once: they would spill
         load_params<T, V>(a, a.w, at[k].col, 1.0f, w[k]);
@@ -414,6 +417,8 @@ __device__ __forceinline__ void backward_of_rows(const NormArgs& a, int group, i
     vec next_x[K], next_dy[K];
     float2 next_s = *(const float2*)(a.stats + 2 * row);
     constexpr bool AHEAD = TPR < 1024;  // the next row is on its way while one is computed
+    // with one vector to a thread the branch costs more than it leaves out; in the largest groups with GELU there is no register for it
+    constexpr bool LEAVE = K > 1 && !(TPR == 1024 && V == 8 && ACT != RBL_ACT_NONE);
     if (AHEAD) {
       load_row<T, V, STREAM>(next_x, a.x, row * a.x_stride, at);
       load_row<T, V, STREAM>(next_dy, a.dy, row * a.dy_stride, at);
@@ -441,6 +446,7 @@ __device__ __forceinline__ void backward_of_rows(const NormArgs& a, int group, i
       float s[2] = {0, 0};
 #pragma unroll
       for (int k = 0; k < K; ++k) {
+        if (LEAVE && !at[k].busy) continue;
         if (!KEEP) {
           __builtin_amdgcn_sched_barrier(0);
           load_params<T, V>(a, a.w, at[k].col, 1.0f, w[k]);
@@ -481,6 +487,7 @@ __device__ __forceinline__ void backward_of_rows(const NormArgs& a, int group, i
         T* dx = (T*)a.dx + row * a.cols;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
+          if (LEAVE && !at[k].busy) continue;
           vec out;
 #pragma unroll
           for (int i = 0; i < V; ++i) out[i] = (T)(r * (g[k][i] - __builtin_fmaf(h[k][i], q, p)));
