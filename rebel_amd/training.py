@@ -6,7 +6,10 @@ behind it) and between the backward pass and the optimizer (the gradients' norm 
     train_step                one step of a trainer: Net2(native=True) forward, loss, backward, clipping, optimizer
 
 Everything runs on torch's current stream and can be captured into a HIP graph; there is no CPU path.  A refused argument
-raises ValueError, a failed launch RuntimeError.
+raises ValueError, a failed launch RuntimeError.  Results repeat bit by bit: no sum depends on timing.
+
+Capturing a backward pass: no graph that was made outside the capture may still hold a leaf of it (layer_norm refuses such a
+leaf; delete the outputs of the warm-up first).
 """
 import torch
 from torch import nn
@@ -23,10 +26,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, activation=None):
     """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension of x; activation "gelu": x/2 (1 + erf(x / sqrt 2))
     of that, in the same pass.
 
-    x: float32, float16 or bfloat16 on the GPU, any leading dimensions.  weight, bias: None, or [x.size(-1)] of x's type or
-    float32.  The result has x's type; statistics, sums and the activation are computed in 32 bits.  Differentiable once in x,
-    weight and bias.  Rows may lie at any one distance from each other; a layout that one row distance does not describe is
-    copied first.
+    x: float32, float16 or bfloat16 on the GPU, any leading dimensions, up to 2^30 columns.  weight, bias: None, or
+    [x.size(-1)] of x's type or float32.  The result has x's type; statistics, sums and the activation are computed in 32 bits.
+    Differentiable once in x, weight and bias.  Rows may lie at any one distance from each other; a layout that one row distance
+    does not describe is copied first.
     """
     if activation not in ACTIVATIONS:
         raise ValueError(f"layer_norm: activation must be None or 'gelu', not {activation!r}")
@@ -36,7 +39,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, activation=None):
 
 
 class LayerNorm(nn.Module):
-    """nn.LayerNorm over the last dimension (same parameters, same state_dict) on layer_norm; `activation` as there.
+    """layer_norm as a module, with its parameters under the usual names (weight, bias: the state_dict of a net that is trained
+    with it loads anywhere); `activation` as there.
 
     A scripted or traced copy holds torch's own operators, so that a saved TorchScript file needs nothing of this package.
     """
@@ -81,9 +85,9 @@ def grad_norm(tensors, norm_type=2.0):
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """Scales the gradients of `parameters` in place by min(1, max_norm / (norm + 1e-6)) and returns grad_norm of them before.
 
-    As torch.nn.utils.clip_grad_norm_: parameters without a gradient are passed over, no gradient at all gives tensor(0.), a norm
-    that is not finite scales all the same unless error_if_nonfinite (which waits for the norm on the host).  Gradients that
-    share memory are refused.
+    Parameters without a gradient are passed over; no gradient at all gives tensor(0.).  A norm that is not finite scales all the
+    same (the formula's zeros and NaN), unless error_if_nonfinite, which waits for the norm on the host and raises RuntimeError
+    with the gradients as they were.  Gradients that share memory are refused; one with gaps between its values is copied.
     """
     return _train.clip_grad_norm(_as_list(parameters), float(max_norm), float(norm_type), error_if_nonfinite)
 
