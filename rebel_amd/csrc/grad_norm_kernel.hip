@@ -412,7 +412,8 @@ int rbl_grad_scale(int device, const rbl_grad* grads, int n, double max_norm, co
     rbl::ClipArgs a{};
     a.norm_in = norm_dev;
     a.max_norm = max_norm;
-    rbl::for_tables((const void*)rbl::grad_scale_kernel<0, rbl::GradTable>, (const void*)rbl::grad_scale_kernel<0, rbl::ChunkTable>, grads, n, a, rbl::plan_of(grads, n), true, (hipStream_t)stream);
+    rbl::for_tables((const void*)rbl::grad_scale_kernel<0, rbl::GradTable>, (const void*)rbl::grad_scale_kernel<0, rbl::ChunkTable>,
+                    grads, n, a, rbl::plan_of(grads, n), true, (hipStream_t)stream);
   });
 }
 

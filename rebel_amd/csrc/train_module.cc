@@ -99,6 +99,8 @@ void check_arguments(const Tensor& x, const Tensor& w, const Tensor& b) {
   require(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(),
               "layer_norm: weight and bias must have one type");
   require(x.layout() == at::kStrided, "layer_norm: x must be a dense tensor");
+  for (const Tensor* t : {&x, &w, &b})
+    require(!t->defined() || !t->_fw_grad(0).defined(), "layer_norm: forward-mode derivatives are not supported");
   require(x.is_cuda(), "layer_norm: x must be on the GPU: there is no CPU path");
 }
 
@@ -144,8 +146,9 @@ class LayerNormBackward : public torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     torch::autograd::variable_list out(3);
     if (!grads[0].defined()) return out;
-    at::AutoDispatchBelowADInplaceOrView plain;
+    // a hook of the saved tensors may run operations with gradients here (recomputation), so not below autograd
     const Tensor x = x_.unpack(), w = w_.unpack(), b = b_.unpack();
+    at::AutoDispatchBelowADInplaceOrView plain;
     c10::DeviceGuard guard(x.device());
     const Tensor dy = with_rows(grads[0]);
     rbl_layer_norm_shape s = shape_of(x, w, b, eps_, activation_);
@@ -192,9 +195,9 @@ Tensor layer_norm(const Tensor& x_in, const OptTensor& weight, const OptTensor& 
   Tensor stats;
   Tensor y = forward(x, w, b, eps, activation, &stats);
   const auto param_type = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : at::kFloat;
+  plain.reset();  // before the tensors are saved: their hooks may run operations with gradients
   auto node = std::shared_ptr<LayerNormBackward>(new LayerNormBackward(x, w, b, stats, eps, activation, param_type),
                                                  torch::autograd::deleteNode);
-  plain.reset();
   node->set_next_edges(torch::autograd::collect_next_edges(x_in, w_in, b_in));
   torch::autograd::set_history(y, node);
   return y;
@@ -283,9 +286,13 @@ std::vector<const Tensor*> tensors_of(const py::list& list) {
 }
 
 Tensor grad_norm(const py::list& tensors, double norm_type) {
+  const auto list = tensors_of(tensors);
+  if (at::GradMode::is_enabled())
+    for (const Tensor* t : list)
+      require(!t->requires_grad(), "gradients: grad_norm has no gradient of its own; detach the tensors, or call it under no_grad");
   at::NoGradGuard no_grad;
   const int kind = norm_kind(norm_type);
-  const Gradients g = gather(tensors_of(tensors), false);
+  const Gradients g = gather(list, false);
   return g.any.defined() ? norm_of(g, kind) : at::zeros({});
 }
 

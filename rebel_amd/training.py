@@ -9,7 +9,8 @@ Everything runs on torch's current stream and can be captured into a HIP graph; 
 raises ValueError, a failed launch RuntimeError.  Results repeat bit by bit: no sum depends on timing.
 
 Capturing a backward pass: no graph that was made outside the capture may still hold a leaf of it (layer_norm refuses such a
-leaf; delete the outputs of the warm-up first).
+leaf; delete the outputs of the warm-up first).  torch.cuda.make_graphed_callables keeps its own warm-up's graph and is refused for
+that reason; torch.cuda.graph around a whole step works.
 """
 import torch
 from torch import nn
@@ -28,7 +29,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, activation=None):
 
     x: float32, float16 or bfloat16 on the GPU, any leading dimensions, up to 2^30 columns.  weight, bias: None, or
     [x.size(-1)] of x's type or float32.  The result has x's type; statistics, sums and the activation are computed in 32 bits.
-    Differentiable once in x, weight and bias.  Rows may lie at any one distance from each other; a layout that one row distance
+    Differentiable once, backward, in x, weight and bias.  Rows may lie at any one distance from each other; a layout that one row distance
     does not describe is copied first.
     """
     if activation not in ACTIVATIONS:
@@ -77,7 +78,8 @@ class LayerNorm(nn.Module):
 def grad_norm(tensors, norm_type=2.0):
     """The norm (order 1, 2 or inf) of all values of `tensors` taken as one vector: a float32 scalar on their device.
 
-    Sums are held in 64 bits.  float32, float16 and bfloat16 tensors may be mixed; all must be on one GPU.
+    Sums are held in 64 bits.  float32, float16 and bfloat16 tensors may be mixed; all must be on one GPU.  The norm has no gradient:
+    tensors that require one are refused unless under no_grad.
     """
     return _train.grad_norm(_as_list(tensors), float(norm_type))
 

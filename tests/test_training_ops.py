@@ -8,6 +8,7 @@ import math
 
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 from rebel_amd import capi, training
 from rebel_amd.models import Net2
@@ -520,6 +521,24 @@ def test_second_derivative_is_refused():
         torch.autograd.grad(y, x, dy, create_graph=True)
 
 
+@gpu
+def test_what_is_saved_may_be_computed_again_or_kept_elsewhere():
+    """Hooks on the saved tensors: recomputation runs the forward pass, with gradients, inside the backward pass."""
+    torch.manual_seed(3)
+    net = torch.nn.Sequential(training.LayerNorm(48, activation="gelu"), torch.nn.Softsign(), training.LayerNorm(48)).cuda()
+    query = torch.randn(33, 48, device="cuda")
+
+    def grads(run):
+        return torch.autograd.grad(run().square().sum(), list(net.parameters()))
+
+    want = grads(lambda: net(query))
+    again = grads(lambda: checkpoint(net, query, use_reentrant=False))
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+    with torch.autograd.graph.save_on_cpu():
+        kept = grads(lambda: net(query))
+    assert all(torch.equal(a, b) for a, b in zip(kept, want))
+
+
 # ---------------------------------------------------------------------------------------------------- gradient norm, clipping
 def clip_oracle(tensors, p):
     """The norm in 64 bits (of what the tensors hold now)."""
@@ -724,6 +743,8 @@ def test_layer_norm_refuses():
                       ((x.to_sparse(),), "dense")):
         with pytest.raises(ValueError, match=word):
             training.layer_norm(*bad)
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+        training.layer_norm(torch.autograd.forward_ad.make_dual(x, torch.ones(4, 8)))
     with pytest.raises(ValueError, match="gelu"):
         training.layer_norm(x, activation="tanh")
     with pytest.raises(ValueError, match="gelu"):
@@ -749,6 +770,8 @@ def test_clipping_refuses():
                        (lambda: training.grad_norm([a.grad, a.grad.to("meta")]), "one device")):
         with pytest.raises(ValueError, match=word):
             call()
+    with pytest.raises(ValueError, match="no gradient of its own"):
+        training.grad_norm([a])
     for call in (lambda: training.grad_norm([a.grad, None]), lambda: training.clip_grad_norm_([a, 3.0], 1.0)):
         with pytest.raises(TypeError, match="expected tensors"):
             call()
