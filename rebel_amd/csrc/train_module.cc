@@ -129,12 +129,30 @@ void refuse_foreign_accumulator(const Tensor& t) {
               "capturing (or make it on the capturing stream)");
 }
 
+// What a saved tensor came back as.  A hook of the saved tensors may return anything, and torch compares it with nothing.
+Tensor unpacked(const torch::autograd::SavedVariable& saved, c10::IntArrayRef sizes, at::ScalarType type, at::Device device,
+                const char* what) {
+  Tensor t = saved.unpack();
+  if (!t.defined()) return t;
+  if (t.layout() != at::kStrided || t.sizes() != sizes || t.scalar_type() != type || t.device() != device)
+    throw std::runtime_error(c10::str("layer_norm: a hook of the saved tensors has returned ", what, " as ", t.scalar_type(), " ", t.sizes(),
+                                      " on ", t.device(), ", not as the dense ", type, " ", sizes, " on ", device, " that was saved"));
+  return t;
+}
+
 // The backward pass of one layer_norm call.  Edges: x, weight, bias (empty where one was not given).
 class LayerNormBackward : public torch::autograd::Node {
  public:
   LayerNormBackward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& stats, double eps, int64_t activation,
                     at::ScalarType param_type)
-      : x_(x, false), stats_(stats), eps_(eps), activation_(activation), param_type_(param_type) {
+      : x_(x, false),
+        stats_(stats),
+        sizes_(x.sizes().vec()),
+        type_(x.scalar_type()),
+        device_(x.device()),
+        eps_(eps),
+        activation_(activation),
+        param_type_(param_type) {
     if (w.defined()) w_ = torch::autograd::SavedVariable(w, false);
     // the bias comes back only where the activation's slope depends on it
     if (b.defined() && activation != RBL_ACT_NONE) b_ = torch::autograd::SavedVariable(b, false);
@@ -147,9 +165,13 @@ class LayerNormBackward : public torch::autograd::Node {
     torch::autograd::variable_list out(3);
     if (!grads[0].defined()) return out;
     // a hook of the saved tensors may run operations with gradients here (recomputation), so not below autograd
-    const Tensor x = x_.unpack(), w = w_.unpack(), b = b_.unpack();
+    const Tensor x_back = unpacked(x_, sizes_, type_, device_, "x");
+    const Tensor w_back = unpacked(w_, sizes_.back(), param_type_, device_, "weight");
+    const Tensor b_back = unpacked(b_, sizes_.back(), param_type_, device_, "bias");
     at::AutoDispatchBelowADInplaceOrView plain;
-    c10::DeviceGuard guard(x.device());
+    c10::DeviceGuard guard(device_);
+    // laid out as forward: a copy that a hook has kept need not have the strides of what it copied
+    const Tensor x = with_rows(x_back), w = dense(w_back), b = dense(b_back);
     const Tensor dy = with_rows(grads[0]);
     rbl_layer_norm_shape s = shape_of(x, w, b, eps_, activation_);
     s.param_dtype = element_type(param_type_);
@@ -176,6 +198,9 @@ class LayerNormBackward : public torch::autograd::Node {
  private:
   torch::autograd::SavedVariable x_, w_, b_;
   Tensor stats_;
+  std::vector<int64_t> sizes_;  // of x
+  at::ScalarType type_;
+  at::Device device_;
   double eps_;
   int64_t activation_;
   at::ScalarType param_type_;

@@ -539,6 +539,56 @@ def test_what_is_saved_may_be_computed_again_or_kept_elsewhere():
     assert all(torch.equal(a, b) for a, b in zip(kept, want))
 
 
+@gpu
+def test_what_a_hook_gives_back_may_lie_otherwise():
+    """Saved tensors come back with other strides than they had: windows that were kept on the CPU, a weight and a bias with gaps,
+    rows and columns exchanged in memory."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    line = torch.randn(400, generator=g, device="cuda")
+    w, b = (torch.randn(300, generator=g, device="cuda") for _ in range(2))
+    windows = line.unfold(0, 300, 1)
+    dy = torch.randn(windows.shape, generator=g, device="cuda")
+    plain = run(windows, w, b, dy, "gelu")
+    with torch.autograd.graph.save_on_cpu():
+        kept = run(windows, w, b, dy, "gelu")
+    assert all(torch.equal(p, q) for p, q in zip(kept, plain))
+
+    def spread(t):
+        if t.dim() == 2:
+            return t.t().contiguous().t()
+        return torch.stack([t, torch.full_like(t, math.nan)], 1)[:, 0]
+
+    x = windows.contiguous()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spread):
+        strided = run(x, w, b, dy, "gelu")
+    assert all(torch.equal(p, q) for p, q in zip(strided, plain))
+    ones = torch.ones_like(w)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: ones[:1].expand(300) if t.dim() == 1 else t):
+        repeated = run(x, ones, ones, dy, "gelu")
+    assert all(torch.equal(p, q) for p, q in zip(repeated, run(x, ones, ones, dy, "gelu")))
+
+
+@gpu
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_what_a_hook_gives_back_has_to_be_what_was_saved(which):
+    x, w, b, dy = make(6, 40, torch.float32, torch.float32)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    ways = {"type": lambda t: t.half(), "shape": lambda t: t[..., :39], "one dimension more": lambda t: t[None], "device": lambda t: t.cpu(),
+            "layout": lambda t: t.to_sparse()}
+    for name, way in ways.items():
+        seen = []  # saved in the order x, weight, bias: pack gets each once
+
+        def pack(t):
+            seen.append(t)
+            return len(seen) - 1, t
+
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda k: way(k[1].detach()) if k[0] == which else k[1]):
+            y = training.layer_norm(*leaves, activation="gelu")
+        assert len(seen) == 3
+        with pytest.raises(RuntimeError, match="a hook of the saved tensors has returned " + ("x", "weight", "bias")[which]):
+            torch.autograd.grad(y, leaves, dy)
+
+
 # ---------------------------------------------------------------------------------------------------- gradient norm, clipping
 def clip_oracle(tensors, p):
     """The norm in 64 bits (of what the tensors hold now)."""
