@@ -163,7 +163,11 @@ class LayerNormBackward : public torch::autograd::Node {
       throw std::runtime_error("layer_norm: its gradient has no gradient of its own (create_graph)");
     std::lock_guard<std::mutex> lock(mutex_);
     torch::autograd::variable_list out(3);
+    // torch's engine hands over what fits y; a call of the node itself may hand over anything
     if (!grads[0].defined()) return out;
+    if (grads[0].layout() != at::kStrided || grads[0].sizes() != sizes_ || grads[0].scalar_type() != type_ || grads[0].device() != device_)
+      throw std::runtime_error(c10::str("layer_norm: the gradient of the result must be a dense ", type_, " ", c10::IntArrayRef(sizes_), " on ",
+                                        device_, ", not ", grads[0].scalar_type(), " ", grads[0].sizes(), " on ", grads[0].device()));
     // a hook of the saved tensors may run operations with gradients here (recomputation), so not below autograd
     const Tensor x_back = unpacked(x_, sizes_, type_, device_, "x");
     const Tensor w_back = unpacked(w_, sizes_.back(), param_type_, device_, "weight");

@@ -589,6 +589,22 @@ def test_what_a_hook_gives_back_has_to_be_what_was_saved(which):
             torch.autograd.grad(y, leaves, dy)
 
 
+@gpu
+def test_the_node_itself_called_with_a_gradient():
+    """y.grad_fn(dy) passes torch's engine and its checks by."""
+    x, w, b, dy = make(6, 40, torch.float32, torch.float32)
+    want = run(x, w, b, dy, "gelu")[1:]
+    y = training.layer_norm(*[t.requires_grad_(True) for t in (x, w, b)], activation="gelu")
+    with torch.no_grad():
+        assert all(torch.equal(p, q) for p, q in zip(y.grad_fn(dy), want))
+        for bad in (dy.half(), dy[:5], dy[:, :39], dy[0], dy.cpu(), dy.to_sparse()):
+            with pytest.raises(RuntimeError, match="gradient of the result must be a dense"):
+                y.grad_fn(bad)
+        for bad in ((), (dy, dy)):
+            with pytest.raises(TypeError, match="expected 1 arguments"):
+                y.grad_fn(*bad)
+
+
 # ---------------------------------------------------------------------------------------------------- gradient norm, clipping
 def clip_oracle(tensors, p):
     """The norm in 64 bits (of what the tensors hold now)."""
