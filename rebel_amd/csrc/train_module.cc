@@ -236,6 +236,7 @@ Tensor layer_norm(const Tensor& x_in, const OptTensor& weight, const OptTensor& 
 struct Gradients {
   std::vector<rbl_grad> list;
   std::vector<std::pair<Tensor, Tensor>> copies;  // tensors with gaps: (the tensor, its values side by side)
+  std::vector<const Tensor*> in_place;            // the others, where they are scaled
   Tensor any;
 };
 
@@ -246,7 +247,10 @@ Gradients gather(const std::vector<const Tensor*>& tensors, bool scaled) {
     uintptr_t begin, end;
   };
   std::vector<Span> spans;
-  if (scaled) spans.reserve(tensors.size());
+  if (scaled) {
+    spans.reserve(tensors.size());
+    g.in_place.reserve(tensors.size());
+  }
   for (const Tensor* each : tensors) {
     const Tensor& t = *each;
     require(t.defined(), "gradients: a tensor is undefined");
@@ -274,10 +278,9 @@ Gradients gather(const std::vector<const Tensor*>& tensors, bool scaled) {
     } else if (scaled) {
       const auto at = (uintptr_t)at_data;
       spans.push_back({at, at + t.numel() * t.element_size()});
+      g.in_place.push_back(each);
     }
     g.list.push_back({at_data, t.numel(), type});
-    // as every operation in place: who has saved the tensor for a gradient finds out
-    if (scaled && !t.is_inference()) torch::autograd::impl::bump_version(t);
   }
   std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
   for (size_t i = 1; i < spans.size(); ++i)
@@ -335,19 +338,25 @@ Tensor clip_grad_norm(const py::list& parameters, double max_norm, double norm_t
     const Tensor& grad = p->grad();
     if (grad.defined()) grads.push_back(&grad);
   }
+  std::vector<Tensor> held;  // while other threads may run and give the parameters other gradients
+  if (error_if_nonfinite) {
+    held.reserve(grads.size());
+    for (const Tensor*& t : grads) {
+      held.push_back(*t);
+      t = &held.back();
+    }
+  }
   const Gradients g = gather(grads, true);
   if (!g.any.defined()) return at::zeros({});
   c10::DeviceGuard guard(g.any.device());
   const int n = (int)g.list.size();
   Tensor norm;
-  std::vector<Tensor> held;  // while other threads may run and give the parameters other gradients
   if (error_if_nonfinite) {
     require(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
                 "gradients: error_if_nonfinite looks at the norm on the host, which a capture cannot do");
     norm = norm_of(g, kind);
     float value;
     {
-      for (const Tensor* t : grads) held.push_back(*t);
       py::gil_scoped_release unlocked;
       value = norm.item<float>();
     }
@@ -362,6 +371,9 @@ Tensor clip_grad_norm(const py::list& parameters, double max_norm, double norm_t
                         space.defined() ? space.numel() : 0, stream_of(g.any)));
   }
   for (const auto& c : g.copies) c.first.copy_(c.second);
+  // as every operation in place: who has saved a gradient for another one finds out.  Not where the call was refused above.
+  for (const Tensor* t : g.in_place)
+    if (!t->is_inference()) torch::autograd::impl::bump_version(*t);
   return norm;
 }
 

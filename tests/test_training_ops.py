@@ -731,6 +731,24 @@ def test_clipping_without_gradients():
     assert float(training.grad_norm([torch.empty(0, 4, device="cuda")])) == 0
 
 
+@gpu
+def test_clipping_marks_what_it_has_written():
+    """Versions grow once where gradients are scaled (in place, or copied for their gaps), and not where they are not."""
+    for value in (1.0, math.nan):
+        grads = [torch.full((5,), value, device="cuda"), torch.full((4, 6), value, device="cuda")[:, :3], torch.empty(0, device="cuda")]
+        params = holders(grads)
+        before = [g._version for g in grads]
+        if math.isnan(value):
+            with pytest.raises(RuntimeError, match="not clipped"):
+                training.clip_grad_norm_(params, 1.0, error_if_nonfinite=True)
+            assert [g._version for g in grads] == before
+        for check in (False, True):
+            if not (check and math.isnan(value)):
+                training.clip_grad_norm_(params, 1.0, error_if_nonfinite=check)
+                before = [before[0] + 1, before[1] + 1, before[2]]
+                assert [g._version for g in grads] == before
+
+
 # ---------------------------------------------------------------------------------------------------- as they are used
 def plain_step(net, q, v, bound):
     """Net2's training step in 64 bits from elementary operations (torch's autograd): loss, norm, clipped gradients."""
@@ -846,6 +864,24 @@ def test_clipping_refuses():
     with pytest.raises(ValueError, match="share memory"):
         training.clip_grad_norm_([a, b], 1.0)
     assert training.clip_grad_norm_([], 1.0) == 0 and training.grad_norm([]) == 0
+
+
+def test_a_refused_clipping_leaves_no_mark():
+    """A version that grew though nothing was written would fail the backward pass of whoever has saved the gradient."""
+    one = torch.ones(12)
+    for grads, call, word in (([one[:4], one[2:6]], {}, "share memory"), ([one[:4]], {}, "no CPU path"),
+                              ([one[:4], one[4:].double()], {}, "float32, float16"), ([one[:4], one[4:].to("meta")], {}, "one device"),
+                              ([one[:4], one[4:5].expand(3)], {}, "repeats its memory"), ([one[:4]], {"norm_type": 3.0}, "norm_type"),
+                              ([one[:4]], {"error_if_nonfinite": True}, "no CPU path")):
+        params = []
+        for g in grads:
+            p = torch.nn.Parameter(torch.empty_like(g))
+            p.grad = g
+            params.append(p)
+        before = [g._version for g in grads]
+        with pytest.raises(ValueError, match=word):
+            training.clip_grad_norm_(params, 1.0, **call)
+        assert [g._version for g in grads] == before, word
 
 
 def test_c_entries_refuse():
