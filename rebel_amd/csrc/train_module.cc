@@ -13,6 +13,7 @@
 #include <algorithm>
 #include <cmath>
 #include <mutex>
+#include <numeric>
 #include <optional>
 #include <stdexcept>
 #include <vector>
@@ -240,12 +241,43 @@ struct Gradients {
   Tensor any;
 };
 
+// The memory of a tensor that is scaled
+struct Span {
+  uintptr_t begin, end;
+  const Tensor* tensor;
+};
+
+// Whether two tensors whose spans meet share no element all the same: blocks and steps of one buffer.  Modulo some distance S
+// the bytes of a tensor lie in one arc: the dimensions whose stride S divides drop out, the others and the element's own bytes
+// make its length.  Arcs that do not meet prove it.  S is tried at both tensors' strides and their common divisors: of two blocks of
+// a grid that differ in some dimension, the stride of the next outer one that either has kept separates them.
+bool apart(const Span& a, const Span& b) {
+  std::vector<int64_t> steps;
+  for (const Span* s : {&a, &b})
+    for (int64_t i = 0; i < s->tensor->dim(); ++i)
+      if (s->tensor->size(i) > 1) steps.push_back(s->tensor->stride(i) * s->tensor->element_size());
+  const size_t own = steps.size();
+  for (size_t i = 0; i < own; ++i)
+    for (size_t j = 0; j < i; ++j) steps.push_back(std::gcd(steps[i], steps[j]));
+  const auto arc = [](const Span& s, int64_t step) {
+    int64_t length = s.tensor->element_size();
+    for (int64_t i = 0; i < s.tensor->dim(); ++i) {
+      const int64_t stride = s.tensor->stride(i) * s.tensor->element_size();
+      if (s.tensor->size(i) > 1 && stride % step != 0) length += (s.tensor->size(i) - 1) * stride;
+    }
+    return length;
+  };
+  for (const int64_t step : steps) {
+    const int64_t from_a = (int64_t)(a.begin % step), from_b = (int64_t)(b.begin % step);
+    const int64_t ahead = from_b >= from_a ? from_b - from_a : from_b - from_a + step;  // of b before a
+    if (ahead >= arc(a, step) && ahead + arc(b, step) <= step) return true;
+  }
+  return false;
+}
+
 Gradients gather(const std::vector<const Tensor*>& tensors, bool scaled) {
   Gradients g;
   g.list.reserve(tensors.size());
-  struct Span {
-    uintptr_t begin, end;
-  };
   std::vector<Span> spans;
   if (scaled) {
     spans.reserve(tensors.size());
@@ -266,25 +298,30 @@ Gradients gather(const std::vector<const Tensor*>& tensors, bool scaled) {
       at_data = dense.data_ptr();
       g.copies.emplace_back(t, dense);
       if (scaled) {
-        // the furthest element; no two may share their memory
+        // to the furthest element; no two may share their memory
         int64_t reach = 1;
         for (int64_t i = 0; i < t.dim(); ++i) {
           require(t.size(i) == 1 || t.stride(i) != 0, "gradients: a tensor that repeats its memory cannot be scaled in place");
           reach += (t.size(i) - 1) * t.stride(i);
         }
         const auto at = (uintptr_t)t.data_ptr();
-        spans.push_back({at, at + reach * t.element_size()});
+        spans.push_back({at, at + reach * t.element_size(), each});
       }
     } else if (scaled) {
       const auto at = (uintptr_t)at_data;
-      spans.push_back({at, at + t.numel() * t.element_size()});
+      spans.push_back({at, at + t.numel() * t.element_size(), each});
       g.in_place.push_back(each);
     }
     g.list.push_back({at_data, t.numel(), type});
   }
   std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
-  for (size_t i = 1; i < spans.size(); ++i)
-    require(spans[i].begin >= spans[i - 1].end, "gradients: two of them share memory (the same tensor twice?)");
+  std::vector<const Span*> open;  // those that reach past the begin of the next
+  for (const Span& s : spans) {
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const Span* o) { return o->end <= s.begin; }), open.end());
+    for (const Span* o : open)
+      require(apart(*o, s), "gradients: two of them share memory (the same tensor twice?), or are mixed in it in no regular way");
+    open.push_back(&s);
+  }
   if (g.any.defined()) require(g.any.is_cuda(), "gradients: must be on the GPU: there is no CPU path");
   return g;
 }

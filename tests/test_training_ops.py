@@ -749,6 +749,26 @@ def test_clipping_marks_what_it_has_written():
                 assert [g._version for g in grads] == before
 
 
+@gpu
+@pytest.mark.parametrize("check", [False, True])
+def test_clipping_of_gradients_that_share_a_buffer(check):
+    """Blocks and steps of one matrix, as a fused layer's gradient that is split by columns: each is scaled, and nothing beside them."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for dtype in TYPES.values():
+        whole = torch.randn(50, 41, generator=g, device="cuda").to(dtype)
+        before = whole.clone()
+        parts = lambda m: [m[:, :7], m[:, 7:20], m[:30, 20:30:2], m[:, 21:30:2], m[30:45, 20:29:2], m[3, 30:40]]
+        want = clip_oracle(parts(before), 2)
+        norm = training.clip_grad_norm_(holders(parts(whole)), 0.5, error_if_nonfinite=check)
+        assert abs(norm.double() - want) <= want * U * 1.001
+        touched = torch.zeros(50, 41, dtype=torch.bool, device="cuda")
+        for part in parts(touched):
+            part.fill_(True)
+        assert torch.equal(whole[~touched], before[~touched])
+        v = before.double() * (0.5 / (float(want) + 1e-6))
+        near(whole[touched], (v[touched], v[touched].abs() * 3 * U))
+
+
 # ---------------------------------------------------------------------------------------------------- as they are used
 def plain_step(net, q, v, bound):
     """Net2's training step in 64 bits from elementary operations (torch's autograd): loss, norm, clipped gradients."""
@@ -882,6 +902,65 @@ def test_a_refused_clipping_leaves_no_mark():
         with pytest.raises(ValueError, match=word):
             training.clip_grad_norm_(params, 1.0, **call)
         assert [g._version for g in grads] == before, word
+
+
+def clip_says(a, b):
+    """What a clipping of two gradients on the CPU is refused for."""
+    params = []
+    for g in (a, b):
+        p = torch.nn.Parameter(torch.empty(g.shape, dtype=g.dtype))
+        p.grad = g
+        params.append(p)
+    with pytest.raises(ValueError) as said:
+        training.clip_grad_norm_(params, 1.0)
+    return "memory" if "share memory" in str(said.value) else "fine" if "no CPU path" in str(said.value) else str(said.value)
+
+
+def test_gradients_of_one_buffer_are_told_apart():
+    b = torch.arange(240.0)
+    m, t = b.view(12, 20), b.view(3, 8, 10)
+    fine = [(m[:, :3], m[:, 3:]), (m[:, 3:], m[:, :3]), (m[:, ::2], m[:, 1::2]), (m[::2, :4], m[::3, 4:]), (m[:5, :7], m[2:, 7:]), (m[:, :5], m[2, 5:]),
+            (m.t()[:5], m.t()[5:]), (t[:, :2], t[:, 2:]), (t[:, :, :3], t[:, 1, 3:]), (t[:, 0, :3], t[:, 0, 3:]), (t[:, 1:, :9], t[1, :, 9]),
+            (m[:, :10].reshape(12, 5, 2)[..., 0], m[:, 10:]), (m.view(-1)[::2].view(12, 10), m[:, 1::2]), (m[:, 0], m[:, 1]), (m[3:4, :2], m[3:4, 2:]),
+            (m[:, :2].view(torch.bfloat16), m[:, 2:]), (b[0], b[1:])]
+    for i, (p, q) in enumerate(fine):
+        assert clip_says(p, q) == "fine", i
+    shared = [(m[:, :4], m[:, 3:]), (m[:, ::2], m[:, 2::2]), (m[::2, :4], m[::3, 3:]), (m[:5, :7], m[4:, 6:]), (m[:, :5], m[2, 4:]), (m, m), (m, m.t()),
+              (m[:, :6], m.t()[5:]), (t[:, :3], t[:, 2:]), (t[:, 0, :3], t[:, :, 2:]), (m[:, :2].view(torch.bfloat16)[:, 3:], m[:, 1:]),
+              (m[:, 0], m[5]), (b[:1], b[:1])]
+    for i, (p, q) in enumerate(shared):
+        assert clip_says(p, q) == "memory", i
+
+
+def test_gradients_of_one_buffer_by_chance():
+    """Strided views at random: none that share an element pass; blocks of one grid, with steps, pass if and only if they do not."""
+    import random
+
+    rng = random.Random(7)
+    b = torch.arange(2000.0)
+    for _ in range(1500):
+        views = []
+        for _ in range(2):
+            dims = rng.randrange(1, 4)
+            size, stride = [rng.randrange(1, 6) for _ in range(dims)], [rng.randrange(1, 40) for _ in range(dims)]
+            views.append(b.as_strided(size, stride, rng.randrange(0, 80)))
+        share = bool(set(views[0].reshape(-1).tolist()) & set(views[1].reshape(-1).tolist()))
+        if share:
+            assert clip_says(*views) == "memory", [(v.shape, v.stride(), v.storage_offset()) for v in views]
+    grid = b[:1680].view(5, 7, 6, 8)
+    passed = 0
+    for _ in range(1500):
+        views = []
+        for _ in range(2):
+            at = []
+            for n in grid.shape:
+                lo = rng.randrange(n)
+                at.append(slice(lo, rng.randrange(lo, n) + 1))
+            views.append(grid[tuple(at)])
+        share = bool(set(views[0].reshape(-1).tolist()) & set(views[1].reshape(-1).tolist()))
+        assert clip_says(*views) == ("memory" if share else "fine"), [(v.shape, v.stride(), v.storage_offset()) for v in views]
+        passed += not share
+    assert passed >= 300 and 1500 - passed >= 100  # both sides are met often
 
 
 def test_c_entries_refuse():
