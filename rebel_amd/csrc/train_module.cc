@@ -12,6 +12,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <functional>
 #include <mutex>
 #include <numeric>
 #include <optional>
@@ -247,30 +248,50 @@ struct Span {
   const Tensor* tensor;
 };
 
-// Whether two tensors whose spans meet share no element all the same: blocks and steps of one buffer.  Modulo some distance S
-// the bytes of a tensor lie in one arc: the dimensions whose stride S divides drop out, the others and the element's own bytes
-// make its length.  Arcs that do not meet prove it.  S is tried at both tensors' strides and their common divisors: of two blocks of
-// a grid that differ in some dimension, the stride of the next outer one that either has kept separates them.
-bool apart(const Span& a, const Span& b) {
-  std::vector<int64_t> steps;
-  for (const Span* s : {&a, &b})
-    for (int64_t i = 0; i < s->tensor->dim(); ++i)
-      if (s->tensor->size(i) > 1) steps.push_back(s->tensor->stride(i) * s->tensor->element_size());
-  const size_t own = steps.size();
-  for (size_t i = 0; i < own; ++i)
-    for (size_t j = 0; j < i; ++j) steps.push_back(std::gcd(steps[i], steps[j]));
-  const auto arc = [](const Span& s, int64_t step) {
-    int64_t length = s.tensor->element_size();
-    for (int64_t i = 0; i < s.tensor->dim(); ++i) {
-      const int64_t stride = s.tensor->stride(i) * s.tensor->element_size();
-      if (s.tensor->size(i) > 1 && stride % step != 0) length += (s.tensor->size(i) - 1) * stride;
-    }
-    return length;
+// The bytes of a tensor from its first one: its elements' size and the dimensions of more than one entry, strides in bytes
+struct Lattice {
+  struct Dim {
+    int64_t size, stride;
   };
+  std::vector<Dim> dims;
+  int64_t element;
+
+  explicit Lattice(const Tensor& t) : element((int64_t)t.element_size()) {
+    for (int64_t i = 0; i < t.dim(); ++i)
+      if (t.size(i) > 1) dims.push_back({t.size(i), t.stride(i) * element});
+  }
+  int64_t length() const {
+    int64_t n = element;
+    for (const Dim& d : dims) n += (d.size - 1) * d.stride;
+    return n;
+  }
+  Lattice modulo(int64_t step) const {
+    Lattice rest = *this;
+    rest.dims.erase(std::remove_if(rest.dims.begin(), rest.dims.end(), [&](const Dim& d) { return d.stride % step == 0; }), rest.dims.end());
+    return rest;
+  }
+};
+
+// Whether two tensors share no byte, b beginning `ahead` bytes behind a (or before it): blocks and steps of one buffer can be told
+// apart.  Modulo a distance S the dimensions whose stride S divides drop out.  Where neither of the rests is longer than S, a byte
+// of both would lie in both rests, at the distance `ahead` modulo S or S less: two smaller questions of the same kind.  S is
+// tried at the strides and their common divisors: of two blocks of a grid that differ in some dimension, the stride of the next
+// outer one that either has kept separates them.  `tries` bounds the search; false: not shown.
+bool apart(const Lattice& a, const Lattice& b, int64_t ahead, int& tries) {
+  if (ahead >= a.length() || ahead + b.length() <= 0) return true;
+  std::vector<int64_t> steps;
+  for (const Lattice* l : {&a, &b})
+    for (const auto& d : l->dims) steps.push_back(d.stride);
+  for (size_t i = 0, own = steps.size(); i < own; ++i)
+    for (size_t j = 0; j < i; ++j) steps.push_back(std::gcd(steps[i], steps[j]));
+  std::sort(steps.begin(), steps.end(), std::greater<>());
+  steps.erase(std::unique(steps.begin(), steps.end()), steps.end());
   for (const int64_t step : steps) {
-    const int64_t from_a = (int64_t)(a.begin % step), from_b = (int64_t)(b.begin % step);
-    const int64_t ahead = from_b >= from_a ? from_b - from_a : from_b - from_a + step;  // of b before a
-    if (ahead >= arc(a, step) && ahead + arc(b, step) <= step) return true;
+    if (--tries < 0) return false;
+    const Lattice p = a.modulo(step), q = b.modulo(step);
+    if (p.length() > step || q.length() > step) continue;
+    const int64_t d = (ahead % step + step) % step;
+    if (apart(p, q, d, tries) && apart(p, q, d - step, tries)) return true;
   }
   return false;
 }
@@ -318,8 +339,11 @@ Gradients gather(const std::vector<const Tensor*>& tensors, bool scaled) {
   std::vector<const Span*> open;  // those that reach past the begin of the next
   for (const Span& s : spans) {
     open.erase(std::remove_if(open.begin(), open.end(), [&](const Span* o) { return o->end <= s.begin; }), open.end());
-    for (const Span* o : open)
-      require(apart(*o, s), "gradients: two of them share memory (the same tensor twice?), or are mixed in it in no regular way");
+    for (const Span* o : open) {
+      int tries = 2000;
+      require(apart(Lattice(*o->tensor), Lattice(*s.tensor), (int64_t)(s.begin - o->begin), tries),
+              "gradients: two of them share memory (the same tensor twice?), or are mixed in it in no regular way");
+    }
     open.push_back(&s);
   }
   if (g.any.defined()) require(g.any.is_cuda(), "gradients: must be on the GPU: there is no CPU path");
