@@ -42,6 +42,16 @@ int element_type(at::ScalarType t) {
 
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
+// Whether a dense tensor's elements lie in memory that it has: its storage may have been given back (resized to nothing, as sharded
+// trainers do between uses), and its address is then null, which the C entries take for a parameter that is not given.
+bool in_memory(const Tensor& t) {
+  if (t.numel() == 0) return true;
+  if (!t.has_storage()) return false;
+  int64_t reach = t.storage_offset() + 1;
+  for (int64_t i = 0; i < t.dim(); ++i) reach += (t.size(i) - 1) * t.stride(i);
+  return reach * t.element_size() <= (int64_t)t.storage().nbytes();
+}
+
 // The elements from one row of the last dimension to the next, where all rows lie at one distance; -1 where they do not, or
 // where a row's elements do not lie side by side.
 int64_t row_stride(const Tensor& t) {
@@ -101,8 +111,11 @@ void check_arguments(const Tensor& x, const Tensor& w, const Tensor& b) {
   require(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(),
               "layer_norm: weight and bias must have one type");
   require(x.layout() == at::kStrided, "layer_norm: x must be a dense tensor");
-  for (const Tensor* t : {&x, &w, &b})
+  for (const Tensor* t : {&x, &w, &b}) {
+    require(!t->defined() || t->layout() == at::kStrided, "layer_norm: weight and bias must be dense tensors");
+    require(!t->defined() || in_memory(*t), "layer_norm: x, weight or bias has no memory (its storage is too small)");
     require(!t->defined() || !t->_fw_grad(0).defined(), "layer_norm: forward-mode derivatives are not supported");
+  }
   require(x.is_cuda(), "layer_norm: x must be on the GPU: there is no CPU path");
 }
 
@@ -136,7 +149,7 @@ Tensor unpacked(const torch::autograd::SavedVariable& saved, c10::IntArrayRef si
                 const char* what) {
   Tensor t = saved.unpack();
   if (!t.defined()) return t;
-  if (t.layout() != at::kStrided || t.sizes() != sizes || t.scalar_type() != type || t.device() != device)
+  if (t.layout() != at::kStrided || t.sizes() != sizes || t.scalar_type() != type || t.device() != device || !in_memory(t))
     throw std::runtime_error(c10::str("layer_norm: a hook of the saved tensors has returned ", what, " as ", t.scalar_type(), " ", t.sizes(),
                                       " on ", t.device(), ", not as the dense ", type, " ", sizes, " on ", device, " that was saved"));
   return t;
@@ -167,7 +180,8 @@ class LayerNormBackward : public torch::autograd::Node {
     torch::autograd::variable_list out(3);
     // torch's engine hands over what fits y; a call of the node itself may hand over anything
     if (!grads[0].defined()) return out;
-    if (grads[0].layout() != at::kStrided || grads[0].sizes() != sizes_ || grads[0].scalar_type() != type_ || grads[0].device() != device_)
+    if (grads[0].layout() != at::kStrided || grads[0].sizes() != sizes_ || grads[0].scalar_type() != type_ ||
+        grads[0].device() != device_ || !in_memory(grads[0]))
       throw std::runtime_error(c10::str("layer_norm: the gradient of the result must be a dense ", type_, " ", c10::IntArrayRef(sizes_), " on ",
                                         device_, ", not ", grads[0].scalar_type(), " ", grads[0].sizes(), " on ", grads[0].device()));
     // a hook of the saved tensors may run operations with gradients here (recomputation), so not below autograd
@@ -312,6 +326,7 @@ Gradients gather(const std::vector<const Tensor*>& tensors, bool scaled) {
     require(type >= 0, "gradients: must be float32, float16 or bfloat16, not ", t.scalar_type());
     if (!g.any.defined()) g.any = t;
     require(t.device() == g.any.device(), "gradients: all must be on one device, not on ", g.any.device(), " and ", t.device());
+    require(in_memory(t), "gradients: a tensor has no memory (its storage is too small)");
     if (t.numel() == 0) continue;
     void* at_data = t.data_ptr();
     if (!t.is_non_overlapping_and_dense()) {

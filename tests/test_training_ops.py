@@ -904,6 +904,47 @@ def test_a_refused_clipping_leaves_no_mark():
         assert [g._version for g in grads] == before, word
 
 
+def test_memory_that_was_given_back_is_refused():
+    """A weight whose storage has been resized to nothing has the address 0, which stands for no weight in the C entries."""
+    x, w, b = torch.zeros(4, 8), torch.ones(8), torch.ones(16)[8:]
+    for i in range(3):
+        args = [t.clone() if k != 2 else torch.ones(16)[8:] for k, t in enumerate((x, w, b))]
+        args[i].untyped_storage().resize_(0)
+        with pytest.raises(ValueError, match="no memory"):
+            training.layer_norm(*args)
+        args[i].untyped_storage().resize_(4)  # less than it needs
+        with pytest.raises(ValueError, match="no memory"):
+            training.layer_norm(*args)
+    p = torch.nn.Parameter(torch.zeros(8))
+    p.grad = torch.ones(8)
+    p.grad.untyped_storage().resize_(0)
+    for call in (lambda: training.clip_grad_norm_([p], 1.0), lambda: training.grad_norm([p.grad])):
+        with pytest.raises(ValueError, match="no memory"):
+            call()
+    with pytest.raises(ValueError, match="must be dense"):
+        training.layer_norm(x, w.to_sparse())
+
+
+@gpu
+def test_memory_that_was_given_back_is_refused_backward():
+    x, w, b, dy = make(6, 40, torch.float32, torch.float32)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    for i, name in enumerate(("x", "weight", "bias")):
+        y = training.layer_norm(*leaves, activation="gelu")
+        kept = leaves[i].detach().clone()
+        leaves[i].untyped_storage().resize_(0)
+        with pytest.raises(RuntimeError, match="has returned " + name):
+            torch.autograd.grad(y, leaves, dy)
+        leaves[i].untyped_storage().resize_(kept.numel() * 4)
+        with torch.no_grad():
+            leaves[i].data.copy_(kept)
+    y = training.layer_norm(*leaves, activation="gelu")
+    lost = dy.clone()
+    lost.untyped_storage().resize_(0)
+    with pytest.raises(RuntimeError, match="gradient of the result"):
+        torch.autograd.grad(y, leaves, lost)
+
+
 def clip_says(a, b):
     """What a clipping of two gradients on the CPU is refused for."""
     params = []
