@@ -188,6 +188,13 @@ __device__ __forceinline__ void scale_chunk(T* g, int count, float c) {
   if (rest < count) g[rest] = (T)((float)g[rest] * c);
 }
 
+// A factor that has no normal number in f32 (gradients near the type's end): products in f64
+constexpr double kFactorLeast = 0x1p-126;
+template <class T>
+__device__ __forceinline__ void scale_chunk_wide(T* g, int count, double c) {
+  for (int i = threadIdx.x; i < count; i += kThreads) g[i] = (T)(float)((double)(float)g[i] * c);
+}
+
 // NORM 0: the norm is there already
 template <int NORM, class TABLE>
 __global__ __launch_bounds__(kThreads) void grad_scale_kernel(TABLE t, ClipArgs a) {
@@ -203,12 +210,13 @@ __global__ __launch_bounds__(kThreads) void grad_scale_kernel(TABLE t, ClipArgs 
   if (c >= 1.0) return;  // times 1: nothing changes
   // from the last chunk to the first: what the sums read last is what the cache still has
   const Chunk k = chunk_of(t, a, gridDim.x - 1 - blockIdx.x);
+  const auto scale = [&](auto* g) { c < kFactorLeast ? scale_chunk_wide(g, k.count, c) : scale_chunk(g, k.count, (float)c); };
   if (k.type == RBL_F32)
-    scale_chunk((float*)k.data + k.begin, k.count, (float)c);
+    scale((float*)k.data + k.begin);
   else if (k.type == RBL_F16)
-    scale_chunk((_Float16*)k.data + k.begin, k.count, (float)c);
+    scale((_Float16*)k.data + k.begin);
   else
-    scale_chunk((__bf16*)k.data + k.begin, k.count, (float)c);
+    scale((__bf16*)k.data + k.begin);
 }
 
 // The norm from the chunks' sums, for those who ask for it and for a scaling that finds it behind the sums.

@@ -678,6 +678,23 @@ def test_clipping_needs_no_scale():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_clipping_by_a_factor_below_f32(dtype):
+    """Gradients near the type's end under a small bound: the factor is below f32's normal numbers, its products are not."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    for n in (3, 700, 300_001):
+        for bound in (1.0, 1e-3, 1e-9):
+            for p, check in ((2.0, False), (math.inf, False), (math.inf, True)):
+                v = ((torch.rand(n, generator=g, device="cuda") - 0.5) * 2 * 3e38).to(TYPES[dtype])
+                before = v.clone()
+                want = float(clip_oracle([before], p))
+                norm = training.clip_grad_norm_(holders([v]), bound, p, error_if_nonfinite=check)
+                assert norm == torch.tensor(want, dtype=torch.float64).float()
+                w = before.double() * (bound / (want + 1e-6))
+                near(v, (w, w.abs() * 3 * U), (n, bound, p, check))
+
+
+@gpu
 @pytest.mark.parametrize("p", [1.0, 2.0, math.inf])
 def test_clipping_of_what_is_not_finite(p):
     """As the formula: an infinite norm gives the factor 0 (and inf * 0 = NaN), a NaN reaches everything."""
