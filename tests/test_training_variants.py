@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from rebel_amd import capi, training
-from tests.test_training_ops import EPS, TYPES, U, make, near, oracle, run
+from tests.test_training_ops import EPS, TYPES, U, clip_oracle, holders, make, near, oracle, run
 
 gpu = pytest.mark.gpu
 SIZE = {"f32": 4, "f16": 2, "bf16": 2}
@@ -205,3 +205,89 @@ def test_layer_norm_variants_past_the_caches(cols, dtype):
         x, w, b, dy = make(rows, cols, TYPES[dtype], torch.float32)
         compare(x, w, b, dy, gelu, run(x, w, b, dy, "gelu" if gelu else None), Backward(rows, cols, dtype).depth())
     torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------------------------------------------- gradient norm, clipping
+def chunks_of(grads):
+    """How many chunks the library cuts a set into: one f64 for each, and one more."""
+    a = (capi.Grad * len(grads))(*[capi.Grad(16, n, CODE[t]) for n, t in grads])
+    return capi.lib().rbl_grad_workspace(a, len(grads)) // 8 - 1
+
+
+def mixed(count, size):
+    return [(size(i), ("f32", "bf16", "f16")[i % 3]) for i in range(count)]
+
+
+MB = 1 << 20
+# name: (tensors, chunks).  Up to 320 chunks travel in the arguments of one launch; up to 4096 sums are added up by every workgroup of the
+# scaling, more by a launch of their own; chunks grow from 8 KB to 128 KB, stay there, and grow again from 1 GB on.
+SETS = {"320 chunks": (mixed(320, lambda i: 1 + i), 320), "321 chunks": (mixed(321, lambda i: 1 + i), 321),
+        "4096 chunks": (mixed(4096, lambda i: 1 + i % 50), 4096), "4097 chunks": (mixed(4097, lambda i: 1 + i % 50), 4097),
+        "5000 tensors": (mixed(5000, lambda i: 1 + 7 * i % 2500), None), "100 MB": (mixed(3, lambda i: 12 * MB + 5 * i + 1), None),
+        "200 MB": (mixed(4, lambda i: 20 * MB + 3 * i + 1), None), "600 MB": (mixed(5, lambda i: 48 * MB + i), None),
+        "1200 MB": (mixed(7, lambda i: 72 * MB + 3 * i), None)}
+
+
+def test_every_way_of_clipping_has_a_set():
+    for name, (grads, chunks) in SETS.items():
+        assert chunks in (None, chunks_of(grads)), name
+    of = {name: chunks_of(grads) for name, (grads, _) in SETS.items()}
+    size = {name: sum(n * SIZE[t] for n, t in grads) for name, (grads, _) in SETS.items()}
+    assert of["5000 tensors"] > 4096 and of["600 MB"] > 4096 and of["1200 MB"] > 4096
+    # bytes to a chunk, by what the last chunks of a few large tensors leave over
+    chunk = {name: next(1 << k for k in range(13, 40) if sum(ceil(n * SIZE[t], 1 << k) for n, t in SETS[name][0]) == of[name])
+             for name in ("100 MB", "200 MB", "600 MB", "1200 MB")}
+    assert chunk == {"100 MB": 64 << 10, "200 MB": 128 << 10, "600 MB": 128 << 10, "1200 MB": 256 << 10}, (chunk, size)
+
+
+def values(name):
+    g = torch.Generator(device="cuda").manual_seed(len(name))
+    return [torch.randn(n, generator=g, device="cuda").to(TYPES[t]) for n, t in SETS[name][0]]
+
+
+@gpu
+@pytest.mark.parametrize("p", [1.0, 2.0, math.inf])
+@pytest.mark.parametrize("name", list(SETS))
+def test_clipping_of_many_chunks(name, p):
+    grads = values(name)
+    want = float(clip_oracle(grads, p))
+    norm = training.grad_norm(grads, p)
+    assert abs(float(norm) - want) <= want * U * 1.001
+    before = [v.clone() for v in grads]
+    assert torch.equal(training.clip_grad_norm_(holders(grads), 2 * want, p), norm)
+    assert all(torch.equal(x, y) for x, y in zip(before, grads))
+    bound = 0.37 * want
+    for check in (False, True):
+        held = [v.clone() for v in grads]
+        assert torch.equal(training.clip_grad_norm_(holders(held), bound, p, error_if_nonfinite=check), norm)
+        # as one vector of each type: the factor's rounding, the product's and (check) the norm's
+        for t in TYPES.values():
+            v = [x.reshape(-1) for x in before if x.dtype == t]
+            got = [x.reshape(-1) for x in held if x.dtype == t]
+            if v:
+                w = torch.cat(v).double() * (bound / (want + 1e-6))
+                near(torch.cat(got), (w, w.abs() * 3 * U), (name, check))
+
+
+@gpu
+@pytest.mark.parametrize("name", ["320 chunks", "4096 chunks", "4097 chunks", "5000 tensors"])
+def test_clipping_keeps_to_its_workspace(name):
+    """The C entries with a workspace of exactly the bytes they ask for, between guards."""
+    L = capi.lib()
+    for norm, p in ((capi.NORM_1, 1.0), (capi.NORM_2, 2.0), (capi.NORM_INF, math.inf)):
+        grads = values(name)
+        want = float(clip_oracle(grads, p))
+        a = (capi.Grad * len(grads))(*[capi.Grad(v.data_ptr(), v.numel(), CODE[t]) for v, (_, t) in zip(grads, SETS[name][0])])
+        need = L.rbl_grad_workspace(a, len(grads))
+        space = torch.full((need + 1024,), 9, dtype=torch.uint8, device="cuda")
+        out = torch.full((3,), 7.0, device="cuda")
+        at, st = space.data_ptr() + 512, torch.cuda.current_stream().cuda_stream
+        for call in (lambda: L.rbl_grad_norm(0, a, len(grads), norm, out.data_ptr() + 4, at, need, st),
+                     lambda: L.rbl_grad_clip(0, a, len(grads), norm, 0.25 * want, out.data_ptr() + 4, at, need, st)):
+            out[1] = 0
+            capi._check(call())
+            assert abs(float(out[1]) - want) <= want * U * 1.001 and out[0] == 7 and out[2] == 7
+            assert bool((space[:512] == 9).all()) and bool((space[512 + need:] == 9).all())
+        # half a step of the type at every element (bf16's the coarsest; half of f16's subnormal step), as one vector
+        clipped = float(clip_oracle(grads, p))
+        assert abs(clipped - 0.25 * want) <= 0.25 * want * (2 ** -8 + 3 * U) + 1e-6 + sum(n for n, _ in SETS[name][0]) * 2 ** -25
