@@ -40,9 +40,9 @@ inline unsigned even_grid(int64_t need, int64_t resident) {
   return (unsigned)((need + rounds - 1) / rounds);
 }
 
-// Workgroup size of the backward kernel, as forward.  Eight wavefronts to a CU are the best number at every width (more slow the
-// three streams down and leave more partial sums: 270336 x 256 f32 + GELU 150 us with 8, 167 with 16, 178 with 32; 8192 x 4096 bf16
-// 44 / 48 / 56 us).
+// Workgroup size of the backward kernel, as forward.  Eight wavefronts to a CU are the best number for rows that are bound by memory
+// (more slow the three streams down and leave more partial sums: back to back, 270336 x 256 f32 + GELU 150 us with 8, 167 with 16, 178
+// with 32; 8192 x 4096 bf16 44 / 48 / 56 us).  16-bit rows with GELU, which are bound by issue, were not measured with more.
 constexpr int backward_threads(int tpr) { return tpr <= 64 ? 256 : tpr; }
 constexpr int kBackwardWaves = 8;
 
@@ -54,8 +54,11 @@ struct BackwardPlan {
   bool few;  // so few rows that the parameters' gradients are taken from x and dy in the same launch
 };
 
-// Few rows: 512 x 256 f32 + GELU takes 5.0 us in one launch (5.9 with partial sums), 512 x 4096 11.7 (13.2), 24 x 65537 14 (20); with
-// more of them the second reading costs more than it saves (1024 x 256 7.6 (6.3), 512 x 8192 22.9 (17.2)).
+// Few rows, f32, in one launch against two (the sum of both kernels; the second launch's gap comes on top), us, behind a forward pass:
+//     512 x 256 + GELU 6.7 / 7.6    640 x 256 7.5 / 7.9    768 x 256 8.6 / 7.6    1024 x 256 10.6 / 7.7
+//     512 x 4096 10.0 / 12.9    512 x 8192 19.6 / 15.4    256 x 16384 22.2 / 22.6    24 x 65537 9.8 / 18.5 (the second of two kernels)
+// Back to back 512 x 256 takes 5.4 / 7.6, 768 x 256 6.7 / 7.4, 1024 x 256 8.0 / 7.6.  With more rows the second reading costs more than
+// it saves.
 constexpr int64_t kFewRows = 512, kFewElements = 1 << 21;
 
 inline BackwardPlan backward_plan(const rbl_layer_norm_shape& s) {
@@ -68,7 +71,7 @@ inline BackwardPlan backward_plan(const rbl_layer_norm_shape& s) {
     const int nt = backward_threads(p.tpr);
     const int64_t need = (s.rows * p.tpr + nt - 1) / nt;
     // Threads past the row's end have nothing to load.  16-bit rows have one vector to a thread, and make up for them with more
-    // workgroups (65536 x 1280 bf16 113 us instead of 131, 32768 x 2560 106 instead of 126); f32 rows have two, and are slower for it.
+    // workgroups (65536 x 1280 bf16 without GELU 113 us instead of 131, 32768 x 2560 106 instead of 126); f32 rows have two, and are slower for it.
     const int64_t threads = kBackwardWaves * 64;
     int64_t per_cu = threads / nt;
     if (s.dtype != RBL_F32 && s.cols <= 4096) per_cu = (threads * p.tpr * 8 + nt * s.cols / 2) / (nt * s.cols);

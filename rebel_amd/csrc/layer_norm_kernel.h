@@ -8,10 +8,20 @@
 //
 // h is computed again from x and the two statistics of the row, so nothing else is kept between the passes.
 //
-// All of it is bound by memory where the tensors are large: 8 to 15 instructions an element, 20 more for the GELU, whose
-// exponential and reciprocal count fourfold.  (f32 + GELU hides behind the memory; 16-bit rows + GELU do not: 8192 x 12000 bf16
-// takes 134 us with it and 87 without.)  So a row is read once and stays in registers, and a thread has as many of its elements
-// as fit there: what is done once per row and thread (two sums over the group, the statistics) is then done least often.
+// Large tensors are bound by memory, but for 16-bit rows with GELU.  Counted in the loops over the rows (bf16, branches and
+// all), an element takes 14 to 20 issue slots forward and 16 to 28 backward; with GELU, whose exponential and reciprocal count fourfold,
+// 38 to 44 and 47 to 66.  At 39 T lane slots a second (256 CUs, 64 lanes, 2.4 GHz) f32 + GELU hides behind the memory.  16-bit rows
+// + GELU do not.  bf16, us, with GELU / the time of its slots / without GELU:
+//     forward     8192 x 4096 39 / 36 / 27    8192 x 12000 122 / 110 / 80    65536 x 1280 125 / 92 / 62
+//     backward    8192 x 4096 49 / 48 / 38    8192 x 12000 202 / 122 / 142    65536 x 1280 187 / 128 / 115
+// What goes beyond the slots in the two widths that are no power of two: threads past the row's end (27 and 37 % of them) take part in
+// the statistics, and backward two wavefronts to a SIMD have to cover the chains through exponential and reciprocal.
+//
+// So a row is read once and stays in registers, and a thread has as many of its elements as fit there: what is done once per row
+// and thread (two sums over the group, the statistics) is then done least often.
+//
+// Times here and in layer_norm.h: rocprofv3's durations of the kernels, median of 30 passes over three sets of inputs in turn; "back to
+// back": 200 calls of the C entry with nothing between them.
 //
 // The element types are compiled apart (layer_norm_f32.hip, layer_norm_f16.hip, layer_norm_bf16.hip); layer_norm.hip holds the C
 // entries.
@@ -209,7 +219,7 @@ constexpr int forward_threads() { return TPR <= 64 ? 256 : TPR; }
 // Forward, a row in the registers of TPR threads (K vectors of V elements each): read once, written once.  As many workgroups as
 // the chip holds, each with the same number of rows, the parameters in registers and the next row on its way.  Bound by memory:
 // 270336 x 256 f32 + GELU 103 us (5.4 TB/s; with 4 elements to a thread instead of 16 it was 149), 8192 x 4096 bf16 23.4 us (5.7),
-// 32768 x 8192 bf16 178 us (6.0).  One row of 256: 2.2 us, a load, two sums and a store one after the other.
+// 32768 x 8192 bf16 178 us (6.0).  One row of 256: 2.6 us, a load, two sums and a store one after the other.
 template <class T, int V, int TPR, int K, bool EVEN, int ACT, bool STREAM>
 __global__ __launch_bounds__(forward_threads<TPR>()) void layer_norm_forward_kernel(NormArgs a) {
   constexpr int NT = forward_threads<TPR>(), RPB = NT / TPR;
@@ -268,7 +278,7 @@ __global__ __launch_bounds__(forward_threads<TPR>()) void layer_norm_forward_ker
 
 // Rows that are longer than a workgroup's registers: chunks of kChunkK vectors to a thread, each with its own mean and sum of
 // squared deviations, which the second kernel joins (Chan's formula) before it normalises its chunk.  x is read twice: 2000 x 65537
-// f32 306 us (5.1 TB/s of three passes), 24 x 65537 3.8 + 5.6 us.  Batches of rows small enough for the second reading to come
+// f32 109 + 192 us (5.2 TB/s of three passes), 24 x 65537 4.1 + 5.8 us.  Batches of rows small enough for the second reading to come
 // from the 256 MB cache were not faster (4096 x 65537: 608 us in one, 626 in batches of 128 MB).
 template <int V>
 constexpr int chunk_cols() { return kThreads * kChunkK * V; }
@@ -379,8 +389,8 @@ __device__ __forceinline__ void put_sums(float* out, const float (&v)[V], int sk
 
 // Backward, a row in the registers of TPR threads: x and dy are read once, dx is written, and (SUMS) g h and g are summed up over
 // the rows of the workgroup, in registers (rows of 1024 threads: in LDS, each thread its own 16-byte cells); the workgroups' sums
-// are joined by layer_norm_sums_kernel.  Bound by memory: 270336 x 256 f32 + GELU 150 us (5.5 TB/s), 32768 x 8192 bf16 265 us (6.1),
-// 8192 x 16384 bf16 173 us (4.7).  Workgroup `group` of `groups`.
+// are joined by layer_norm_sums_kernel.  Bound by memory: 270336 x 256 f32 + GELU 160 to 170 us behind a forward pass and
+// 148 back to back (4.9 to 5.6 TB/s), 32768 x 8192 bf16 264 us (6.1), 8192 x 16384 bf16 178 to 188 us (4.3 to 4.5).  Workgroup `group` of `groups`.
 template <class T, int V, int TPR, int K, bool EVEN, int ACT, bool SUMS, bool STREAM>
 __device__ __forceinline__ void backward_of_rows(const NormArgs& a, int group, int groups) {
   constexpr int NT = backward_threads(TPR), RPB = NT / TPR;
@@ -789,9 +799,12 @@ __device__ __forceinline__ void backward_of_chunk(const NormArgs& a, int block, 
   }
 }
 
-// A tensor of this size leaves nothing in the cache of 256 MB that its next reader could use: past the caches, 32768 x 8192 bf16
-// takes 181 instead of 197 us forward, 276 instead of 292 us backward.  With smaller ones the reader would pay (16384 x 2048 bf16
-// and a pass over its result: 48 instead of 43 us).
+// A tensor of this size leaves little in the cache of 256 MB that its next reader could use.  bf16 rows of 4096, past the caches
+// against through them, us, forward with an elementwise pass over the result behind it, and backward:
+//     64 MB   52 / 49, 38 / 37       128 MB   96 / 94, 72 / 80      192 MB   145 / 145, 104 / 120
+//    256 MB  202 / 202, 138 / 156    384 MB  297 / 308, 200 / 226    512 MB   400 / 408, 267 / 298
+// (32768 x 8192, 512 MB: 397 / 398, 274 / 303.)  Forward, the reader pays for it up to 256 MB.  Backward it pays from 128 MB on by itself,
+// which this one threshold leaves; what reads dx was not timed.
 constexpr int64_t kStreamBytes = (int64_t)512 << 20;
 template <class T>
 bool beyond_caches(const NormArgs& a) { return a.rows * a.cols * (int64_t)sizeof(T) >= kStreamBytes; }

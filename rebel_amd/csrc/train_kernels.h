@@ -1,7 +1,8 @@
 // rebel_amd/csrc/train_kernels.h -- what the training operators' files share: element types, the C entries' error guard and
 // the reductions of a wavefront.
 //
-// The kernels themselves: layer_norm_kernel.hip (forward and backward), grad_norm_kernel.hip (norm and clipping).
+// The kernels themselves: layer_norm_kernel.h (forward and backward, compiled by layer_norm_{f32,f16,bf16}.hip) and
+// grad_norm_kernel.hip (norm and clipping).
 #pragma once
 #include <hip/hip_runtime.h>
 
