@@ -4,13 +4,14 @@
 //
 // Every tensor is cut into chunks of as many bytes, a workgroup to a chunk.  The first kernel leaves one f64 sum per chunk; the
 // second adds all of them up in every workgroup, in the same order, and scales its chunk (where they are many, a kernel between
-// the two has added them up).  Squares are formed and summed in f64: no
-// gradient that is finite in f32 overflows or vanishes on the way, and the order of the sum does not show in an f32 result.
-// Bound by memory, one reading for the sums and one reading and one writing for the scaling: 400 M f32 in 200 tensors 236 us (6.8 TB/s)
-// and 634 us (5.0 TB/s), 200 M bf16 in 200 tensors 65 us (6.1) and 163 us (4.9), 60 M f16 in 100 tensors 25 us (4.8) and 50 us (4.8).
-// A step whose norm stays under the bound ends after the sums.  Small sets are bound by latency, one load after the other: 3.0 and 3.8 us for the 76 thousand values of a net of two hidden layers of 256, with the chunks
-// themselves in the arguments (3.8 and 4.0 with a search for the tensor).  One workgroup that keeps such a set in its registers took
-// 10.5 us, most of it for its 300 KB through one CU.
+// the two has added them up).  Squares are formed and summed in f64: no gradient that is finite in f32 overflows or vanishes on
+// the way, and the order of the sum does not show in an f32 result.
+// Bound by memory, one reading for the sums and one reading and one writing for the scaling: 400 M f32 in 200 tensors 236 us (6.8
+// TB/s) and 634 us (5.0 TB/s), 200 M bf16 in 200 tensors 65 us (6.1) and 163 us (4.9), 60 M f16 in 100 tensors 25 us (4.8) and 50 us
+// (4.8).  A step whose norm stays under the bound ends after the sums.  Small sets are bound by latency, one load after the other:
+// 3.0 and 3.8 us for the 76 thousand values of a net of two hidden layers of 256, with the chunks themselves in the arguments (3.8
+// and 4.0 with a search for the tensor).  One workgroup that keeps such a set in its registers took 10.5 us, most of it for its 300 KB
+// through one CU.
 //
 // The table of tensors travels in the kernel's arguments, as many as fit in 4 KB to a launch: nothing is copied to the device
 // beforehand, so a captured call replays with the pointers it was captured with and needs no memory of the host's.

@@ -42,14 +42,15 @@ int element_type(at::ScalarType t) {
 
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
-// Whether a dense tensor's elements lie in memory that it has: its storage may have been given back (resized to nothing, as sharded
-// trainers do between uses), and its address is then null, which the C entries take for a parameter that is not given.
+// Whether a dense tensor's elements lie in memory that it has.  Its storage may have been given back (resized to nothing, as sharded
+// trainers do between uses), or a subclass that wraps other tensors may have none: the address is then null, which the C entries
+// take for a parameter that is not given.
 bool in_memory(const Tensor& t) {
   if (t.numel() == 0) return true;
   if (!t.has_storage()) return false;
   int64_t reach = t.storage_offset() + 1;
   for (int64_t i = 0; i < t.dim(); ++i) reach += (t.size(i) - 1) * t.stride(i);
-  return reach * t.element_size() <= (int64_t)t.storage().nbytes();
+  return reach * t.element_size() <= (int64_t)t.storage().nbytes() && t.storage().data();
 }
 
 // The elements from one row of the last dimension to the next, where all rows lie at one distance; -1 where they do not, or
@@ -113,7 +114,7 @@ void check_arguments(const Tensor& x, const Tensor& w, const Tensor& b) {
   require(x.layout() == at::kStrided, "layer_norm: x must be a dense tensor");
   for (const Tensor* t : {&x, &w, &b}) {
     require(!t->defined() || t->layout() == at::kStrided, "layer_norm: weight and bias must be dense tensors");
-    require(!t->defined() || in_memory(*t), "layer_norm: x, weight or bias has no memory (its storage is too small)");
+    require(!t->defined() || in_memory(*t), "layer_norm: x, weight or bias has no memory of its own, or too little");
     require(!t->defined() || !t->_fw_grad(0).defined(), "layer_norm: forward-mode derivatives are not supported");
   }
   require(x.is_cuda(), "layer_norm: x must be on the GPU: there is no CPU path");
@@ -326,7 +327,7 @@ Gradients gather(const std::vector<const Tensor*>& tensors, bool scaled) {
     require(type >= 0, "gradients: must be float32, float16 or bfloat16, not ", t.scalar_type());
     if (!g.any.defined()) g.any = t;
     require(t.device() == g.any.device(), "gradients: all must be on one device, not on ", g.any.device(), " and ", t.device());
-    require(in_memory(t), "gradients: a tensor has no memory (its storage is too small)");
+    require(in_memory(t), "gradients: a tensor has no memory of its own, or too little");
     if (t.numel() == 0) continue;
     void* at_data = t.data_ptr();
     if (!t.is_non_overlapping_and_dense()) {

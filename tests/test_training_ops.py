@@ -942,6 +942,29 @@ def test_memory_that_was_given_back_is_refused():
         training.layer_norm(x, w.to_sparse())
 
 
+class Wrapped(torch.Tensor):
+    """A tensor that holds another and has no memory of its own."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(cls, t.size(), dtype=t.dtype, device=t.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, f, types, args=(), kwargs=None):
+        raise AssertionError(f)
+
+
+def test_tensors_without_memory_of_their_own_are_refused():
+    x, w = torch.zeros(4, 8), torch.ones(8)
+    for args in ((x, Wrapped(w)), (x, w, Wrapped(w)), (Wrapped(x), w)):
+        with pytest.raises(ValueError, match="no memory"):
+            training.layer_norm(*args)
+    with pytest.raises(ValueError, match="no memory"):
+        training.grad_norm([w, Wrapped(w)])
+    with torch.no_grad(), pytest.raises(ValueError, match="no memory"):
+        torch.func.vmap(training.layer_norm)(x)
+
+
 @gpu
 def test_memory_that_was_given_back_is_refused_backward():
     x, w, b, dy = make(6, 40, torch.float32, torch.float32)
