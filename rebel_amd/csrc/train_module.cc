@@ -17,6 +17,7 @@
 #include <numeric>
 #include <optional>
 #include <stdexcept>
+#include <utility>
 #include <vector>
 
 #include "../../include/rebel_hip.h"
@@ -48,9 +49,11 @@ void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t
 bool in_memory(const Tensor& t) {
   if (t.numel() == 0) return true;
   if (!t.has_storage()) return false;
+  const c10::StorageImpl& memory = *t.storage().unsafeGetStorageImpl();
+  const auto sizes = t.sizes(), strides = t.strides();
   int64_t reach = t.storage_offset() + 1;
-  for (int64_t i = 0; i < t.dim(); ++i) reach += (t.size(i) - 1) * t.stride(i);
-  return reach * t.element_size() <= (int64_t)t.storage().nbytes() && t.storage().data();
+  for (size_t i = 0; i < sizes.size(); ++i) reach += (sizes[i] - 1) * strides[i];
+  return reach * (int64_t)t.element_size() <= (int64_t)memory.nbytes() && memory.data();
 }
 
 // The elements from one row of the last dimension to the next, where all rows lie at one distance; -1 where they do not, or
@@ -352,6 +355,9 @@ Gradients gather(const std::vector<const Tensor*>& tensors, bool scaled) {
     g.list.push_back({at_data, t.numel(), type});
   }
   std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  uintptr_t reach = 0;
+  const bool apart_all = std::all_of(spans.begin(), spans.end(), [&](const Span& s) { return s.begin >= std::exchange(reach, s.end); });
+  if (apart_all) spans.clear();   // as nearly always
   std::vector<const Span*> open;  // those that reach past the begin of the next
   for (const Span& s : spans) {
     open.erase(std::remove_if(open.begin(), open.end(), [&](const Span* o) { return o->end <= s.begin; }), open.end());

@@ -28,7 +28,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, activation=None):
     of that, in the same pass.
 
     x: float32, float16 or bfloat16 on the GPU, any leading dimensions, up to 2^30 columns.  weight, bias: None, or
-    [x.size(-1)] of x's type or float32.  The result has x's type; statistics, sums and the activation are computed in 32 bits.
+    [x.size(-1)] of x's type or float32.  The result has x's type; statistics, sums and the activation are computed in 32 bits (where a
+    row's sum of values or of squared deviations passes 3e38, it overflows).
     Differentiable once, backward, in x, weight and bias.  Rows may lie at any one distance from each other; a layout that one row distance
     does not describe is copied first.
     """
