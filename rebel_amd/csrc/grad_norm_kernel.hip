@@ -211,7 +211,7 @@ __global__ __launch_bounds__(kThreads) void grad_scale_kernel(TABLE t, ClipArgs 
   if (c >= 1.0) return;  // times 1: nothing changes
   // from the last chunk to the first: what the sums read last is what the cache still has
   const Chunk k = chunk_of(t, a, gridDim.x - 1 - blockIdx.x);
-  const auto scale = [&](auto* g) { c < kFactorLeast ? scale_chunk_wide(g, k.count, c) : scale_chunk(g, k.count, (float)c); };
+  const auto scale = [&](auto* g) { c > 0 && c < kFactorLeast ? scale_chunk_wide(g, k.count, c) : scale_chunk(g, k.count, (float)c); };
   if (k.type == RBL_F32)
     scale((float*)k.data + k.begin);
   else if (k.type == RBL_F16)
