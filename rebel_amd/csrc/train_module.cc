@@ -357,16 +357,26 @@ Gradients gather(const std::vector<const Tensor*>& tensors, bool scaled) {
   std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
   uintptr_t reach = 0;
   const bool apart_all = std::all_of(spans.begin(), spans.end(), [&](const Span& s) { return s.begin >= std::exchange(reach, s.end); });
-  if (apart_all) spans.clear();   // as nearly always
-  std::vector<const Span*> open;  // those that reach past the begin of the next
+  if (apart_all) spans.clear();  // as nearly always
+  struct Open {
+    uintptr_t begin, end;
+    Lattice lattice;
+    int64_t outer, rest;  // the largest stride, and what is left modulo it
+  };
+  std::vector<Open> open;  // those that reach past the begin of the next
   for (const Span& s : spans) {
-    open.erase(std::remove_if(open.begin(), open.end(), [&](const Span* o) { return o->end <= s.begin; }), open.end());
-    for (const Span* o : open) {
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const Open& o) { return o.end <= s.begin; }), open.end());
+    Open mine{s.begin, s.end, Lattice(*s.tensor), 1, 0};
+    for (const auto& d : mine.lattice.dims) mine.outer = std::max(mine.outer, d.stride);
+    mine.rest = mine.lattice.modulo(mine.outer).length();
+    for (const Open& o : open) {
+      const int64_t ahead = (int64_t)(s.begin - o.begin), d = ahead % o.outer;
+      if (mine.outer == o.outer && d >= o.rest && d + mine.rest <= o.outer) continue;  // columns of one matrix: told apart at once
       int tries = 2000;
-      require(apart(Lattice(*o->tensor), Lattice(*s.tensor), (int64_t)(s.begin - o->begin), tries),
+      require(apart(o.lattice, mine.lattice, ahead, tries),
               "gradients: two of them share memory (the same tensor twice?), or are mixed in it in no regular way");
     }
-    open.push_back(&s);
+    open.push_back(std::move(mine));
   }
   if (g.any.defined()) require(g.any.is_cuda(), "gradients: must be on the GPU: there is no CPU path");
   return g;

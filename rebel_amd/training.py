@@ -89,10 +89,10 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     """Scales the gradients of `parameters` in place by min(1, max_norm / (norm + 1e-6)) and returns grad_norm of them before.
 
     Parameters without a gradient are passed over; no gradient at all gives tensor(0.).  A norm that is not finite scales all the
-    same (the formula's zeros and NaN; one that is finite in 64 bits alone is returned as inf and scales by what it is), unless error_if_nonfinite, which waits for the norm on the host and raises RuntimeError
-    with the gradients as they were.  Gradients that share memory are refused; one with gaps between its values is copied.  They may
-    be blocks of one buffer (its columns, say) or every k-th of its rows; where they lie between each other in no such order, they are
-    refused too.
+    same (the formula's zeros and NaN; one that is finite in 64 bits alone is returned as inf and scales by what it is), unless
+    error_if_nonfinite, which waits for the norm on the host and raises RuntimeError with the gradients as they were.  Gradients that
+    share memory are refused; one with gaps between its values is copied.  They may be blocks of one buffer (its columns, say) or every
+    k-th of its rows; where they lie between each other in no such order, they are refused too.
     """
     return _train.clip_grad_norm(_as_list(parameters), float(max_norm), float(norm_type), error_if_nonfinite)
 
